@@ -423,6 +423,91 @@ B200NA_API int b200na_merge(const void* o0, const float* l0, const void* o1, con
                  float* l, int64_t rows, int D, int dtype, b200na_stream_t stream);
 
 /*
+ * Rotary positions over up to three token axes. Channels come in pairs; pair i of axis a turns by
+ *   angle = (origin_a + x_a) * position_scale_a * theta_a^(-2 i / axis_dims_a)
+ * (x_a: the token's coordinate) or, with `positions`, by the given position in place of
+ * origin_a + x_a:   (u, w) -> (u cos - w sin, u sin + w cos); inverse != 0 turns back (the gradient).
+ * Axis a owns axis_dims[a] consecutive channels (even, possibly 0), axis 0 first; channels behind the
+ * last axis are copied. A pair is (i, i + axis_dims_a / 2) of its axis' channels, or neighbours
+ * (2 i, 2 i + 1) when interleaved != 0.
+ * query [B, *shape, Hq, D], key [B, *shape, Hkv, D] or NULL with Hkv = 0 (of `dtype` fp32 / fp16 / bf16;
+ * D <= 256; the channels of a head are contiguous, *_strides holds the element strides of the other
+ * ndim + 2 axes); outputs are contiguous. positions: NULL or contiguous [B or 1, *shape, axes] of
+ * position_type 0 (int32), 1 (int64) or 2 (fp32), B of them when positions_batched != 0; the number of
+ * axes is then free, without positions it is ndim. Angles are worked out in 64 bits and reduced to one
+ * turn before the sine, so far positions lose nothing. Outputs must not overlap the inputs.
+ */
+B200NA_API int b200na_rotary(const void* query, const void* key, void* query_out, void* key_out, int ndim,
+                             const int* shape, int B, int Hq, int Hkv, int D, int dtype,
+                             const int64_t* query_strides, const int64_t* key_strides, int axes,
+                             const int* axis_dims, const double* theta, const double* position_scale,
+                             const int64_t* origin, const void* positions, int position_type,
+                             int positions_batched, int interleaved, int inverse,
+                             b200na_stream_t stream);
+
+/*
+ * A paged key/value cache. Logical token p of sequence b lies in page table[b, p / page_size], slot
+ * p % page_size. A table entry outside [0, pages) is no page: writes to it are dropped, reads of it
+ * give zeros, attention leaves its tokens out. Tables and lengths are int32 in device memory, so a
+ * captured launch follows them.
+ * dtype B200NA_F32 / F16 / BF16, or B200NA_E4M3 with one fp32 scale for each token and head: a row is
+ * value * scale, scale = max(max|x| / 448, 2^-126); a row that holds a NaN or an infinity has the scale
+ * NaN. The channels of a head are contiguous (head_dim <= 256); strides of page, token and head are in
+ * elements of the pool (of the scales: in floats).
+ */
+typedef struct {
+  void* key;
+  void* value;
+  float* key_scale;   /* NULL unless dtype is B200NA_E4M3 */
+  float* value_scale;
+  int64_t key_stride[3], value_stride[3];
+  int64_t key_scale_stride[3], value_scale_stride[3];
+  int64_t pages;
+  int page_size, heads, head_dim, dtype;
+} b200na_kv_cache;
+
+/*
+ * Writes tokens t < counts[b] (all T when counts is NULL) of key / value [B, T, heads, head_dim] at
+ * logical positions start[b] + t (0 + t when start is NULL). dtype: the cache's, or any of fp32 / fp16 /
+ * bf16 for an 8-bit cache. *_strides: element strides of batch, token and head. table: [B, max_pages],
+ * rows table_stride entries apart. Positions that are negative or behind the table are dropped. The
+ * slots that one call writes must be different ones.
+ */
+B200NA_API int b200na_kv_cache_write(const b200na_kv_cache* cache, const void* key, const void* value,
+                                     int B, int T, int dtype, const int64_t* key_strides,
+                                     const int64_t* value_strides, const int* table,
+                                     int64_t table_stride, int max_pages, const int* start,
+                                     const int* counts, b200na_stream_t stream);
+
+/*
+ * Reads tokens start[b] + t, t < length, back into contiguous key / value [B, length, heads, head_dim] of
+ * `dtype` (the cache's, or any of fp32 / fp16 / bf16 for an 8-bit cache); tokens t >= counts[b] are zeros.
+ */
+B200NA_API int b200na_kv_cache_read(const b200na_kv_cache* cache, void* key, void* value, int B, int length,
+                                    int dtype, const int* table, int64_t table_stride, int max_pages,
+                                    const int* start, const int* counts, b200na_stream_t stream);
+
+/*
+ * Attention of the T newest tokens of each sequence over its cache: causal 1-D neighborhood attention
+ * (stride 1) in the form that serving needs. Query t of sequence b stands at p = lengths[b] - T + t and
+ * attends p, p - dilation, ..., `kernel` tokens at most (kernel 0: all), of those that are there. lengths
+ * counts the cached tokens, the T newest included (they are written before). A query that attends
+ * nothing (p < 0, or no page) gives zeros and a logsumexp of -inf.
+ * query: [B, T, Hq, D] of `dtype` fp32 / fp16 / bf16, element strides of batch, token and head; Hq a
+ * multiple of the cache's heads; the cache's dtype is the query's, or B200NA_E4M3. out: contiguous
+ * [B, T, Hq, D]; lse: NULL or contiguous fp32 [B, T, Hq]. workspace:
+ * b200na_na1d_decode_workspace(...) bytes, 16-byte aligned, for this call alone while it runs. Two
+ * launches: parts of equal work whatever the lengths are, and their join.
+ */
+B200NA_API int64_t b200na_na1d_decode_workspace(int B, int T, int Hq, const b200na_kv_cache* cache,
+                                                int max_pages, int kernel, int dilation, int dtype);
+B200NA_API int b200na_na1d_decode(const void* query, const int64_t* query_strides,
+                                  const b200na_kv_cache* cache, void* out, float* lse, int B, int T, int Hq,
+                                  int dtype, const int* table, int64_t table_stride, int max_pages,
+                                  const int* lengths, int kernel, int dilation, float scale,
+                                  void* workspace, b200na_stream_t stream);
+
+/*
  * Device-side status of the tensor-core kernels on the current device. Returns B200NA_OK with
  * *status == 0 if no bounded wait has expired since the last call; otherwise returns
  * B200NA_ERR_KERNEL_TIMEOUT and stores a non-zero diagnostic word (role << 8 | barrier that gave

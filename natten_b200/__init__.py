@@ -20,6 +20,8 @@ from .functional import (BACKEND_NAME, FMHA_BACKEND_NAME, attention, choose_tile
                          token_unpermute_operation)
 
 from .host_io import na_forward_from_host  # noqa: E402
+from .kv_cache import KVCache, kv_cache_read, kv_cache_write, na1d_decode  # noqa: E402
+from .positions import rotary, rotary_axis_dims  # noqa: E402
 from .modules import (NeighborhoodAttention1D, NeighborhoodAttention2D,  # noqa: E402
                       NeighborhoodAttention3D)
 
@@ -27,6 +29,7 @@ __version__ = "0.1.0"
 __all__ = [
     "na1d", "na2d", "na3d", "attention", "merge_attentions", "neighborhood_attention_generic",
     "NeighborhoodAttention1D", "NeighborhoodAttention2D", "NeighborhoodAttention3D",
+    "rotary", "rotary_axis_dims", "KVCache", "kv_cache_write", "kv_cache_read", "na1d_decode",
     "na_forward_from_host", "can_run_b200_fna", "get_configs_for_b200_fna",
     "get_bwd_configs_for_b200_fna", "get_configs_for_b200_fmha", "get_bwd_configs_for_b200_fmha",
     "get_configs_for_cutlass_blackwell_fna", "get_bwd_configs_for_cutlass_blackwell_fna",

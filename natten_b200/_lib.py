@@ -28,8 +28,20 @@ SYMBOLS = (
     "b200na_na_forward_view", "b200na_na_backward_view", "b200na_column_sum", "b200na_column_sum_scratch",
     "b200na_fmha_forward", "b200na_fmha_splits", "b200na_fmha_forward_split",
     "b200na_na_forward", "b200na_na_forward_workspace_bytes", "b200na_na_forward_static", "b200na_na_forward_simt", "b200na_na_backward_simt", "b200na_na_backward_direct", "b200na_merge",
+    "b200na_rotary", "b200na_kv_cache_write", "b200na_kv_cache_read", "b200na_na1d_decode_workspace",
+    "b200na_na1d_decode",
     "b200na_device_status",
 )
+
+
+class KvCacheStruct(ctypes.Structure):
+    """b200na_kv_cache of the C header."""
+    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("key_scale", ctypes.c_void_p),
+                ("value_scale", ctypes.c_void_p), ("key_stride", ctypes.c_int64 * 3),
+                ("value_stride", ctypes.c_int64 * 3), ("key_scale_stride", ctypes.c_int64 * 3),
+                ("value_scale_stride", ctypes.c_int64 * 3), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int), ("heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
 
 
 class NattenB200Error(RuntimeError):
@@ -126,6 +138,23 @@ def _load() -> ctypes.CDLL:
     lib.b200na_merge.restype = c_int
     lib.b200na_merge.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64,
                                  c_int, c_int, c_void_p]
+    i64p, cache = ctypes.POINTER(c_i64), ctypes.POINTER(KvCacheStruct)
+    lib.b200na_rotary.restype = c_int
+    lib.b200na_rotary.argtypes = [c_void_p] * 4 + [c_int, ip] + [c_int] * 5 + [
+        i64p, i64p, c_int, ip, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double), i64p,
+        c_void_p, c_int, c_int, c_int, c_int, c_void_p]
+    lib.b200na_kv_cache_write.restype = c_int
+    lib.b200na_kv_cache_write.argtypes = [cache, c_void_p, c_void_p, c_int, c_int, c_int, i64p, i64p,
+                                          c_void_p, c_i64, c_int, c_void_p, c_void_p, c_void_p]
+    lib.b200na_kv_cache_read.restype = c_int
+    lib.b200na_kv_cache_read.argtypes = [cache, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_i64,
+                                         c_int, c_void_p, c_void_p, c_void_p]
+    lib.b200na_na1d_decode_workspace.restype = c_i64
+    lib.b200na_na1d_decode_workspace.argtypes = [c_int, c_int, c_int, cache] + [c_int] * 4
+    lib.b200na_na1d_decode.restype = c_int
+    lib.b200na_na1d_decode.argtypes = [c_void_p, i64p, cache, c_void_p, c_void_p, c_int, c_int, c_int,
+                                       c_int, c_void_p, c_i64, c_int, c_void_p, c_int, c_int, c_float,
+                                       c_void_p, c_void_p]
     lib.b200na_device_status.restype = c_int
     lib.b200na_device_status.argtypes = [ip]
     return lib
@@ -138,6 +167,14 @@ def ints(x: Optional[Sequence[int]]):
     if x is None:
         return None
     return (ctypes.c_int * len(x))(*[int(v) for v in x])
+
+
+def longs(x: Sequence[int]):
+    return (ctypes.c_int64 * len(x))(*[int(v) for v in x])
+
+
+def doubles(x: Sequence[float]):
+    return (ctypes.c_double * len(x))(*[float(v) for v in x])
 
 
 def strerror(code: int) -> str:

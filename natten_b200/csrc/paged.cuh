@@ -1,0 +1,110 @@
+// Addresses and rows of the paged key/value cache (see b200na_kv_cache in the C header), shared by the
+// kernels that write it, read it back and attend over it.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace b200na {
+
+// e4m3 rows: value * scale. The largest magnitude of a row becomes 448, the type's largest value.
+constexpr float kE4m3Max = 448.f;
+constexpr float kSmallestScale = 1.17549435e-38f;   // 2^-126: its reciprocal is finite
+
+struct PagedPool {
+  void* base;
+  float* scale;                 // fp32 per token and head; nullptr when the pool is not 8-bit
+  int64_t page, token, head;    // strides in elements
+  int64_t s_page, s_token, s_head;
+};
+
+struct PageTable {
+  const int* entry;             // [B, max_pages], rows `stride` entries apart
+  int64_t stride;
+  int max_pages, page_size, shift;   // shift: log2(page_size), -1 when that is no power of two
+  int64_t pages;
+
+  // Page and slot of logical token `p` >= 0 of sequence `b`; page -1 when there is none.
+  __device__ __forceinline__ void split(int64_t p, int64_t* index, int* slot) const {
+    if (shift >= 0) {
+      *index = p >> shift;
+      *slot = (int)(p & (page_size - 1));
+    } else {
+      *index = p / page_size;
+      *slot = (int)(p - *index * page_size);
+    }
+  }
+  __device__ __forceinline__ int64_t page_of(int b, int64_t index) const {
+    if (index < 0 || index >= max_pages) return -1;
+    const int e = entry[b * stride + index];
+    return e >= 0 && e < pages ? e : -1;
+  }
+};
+
+// A stride of an axis of one entry means nothing and is not looked at.
+inline PagedPool paged_pool(const b200na_kv_cache& c, bool value) {
+  const int64_t* s = value ? c.value_stride : c.key_stride;
+  const int64_t* f = value ? c.value_scale_stride : c.key_scale_stride;
+  const bool one[3] = {c.pages <= 1, c.page_size <= 1, c.heads <= 1};
+  PagedPool p{};
+  p.base = value ? c.value : c.key;
+  p.page = one[0] ? 0 : s[0];
+  p.token = one[1] ? 0 : s[1];
+  p.head = one[2] ? 0 : s[2];
+  if (c.dtype == B200NA_E4M3) {
+    p.scale = value ? c.value_scale : c.key_scale;
+    p.s_page = one[0] ? 0 : f[0];
+    p.s_token = one[1] ? 0 : f[1];
+    p.s_head = one[2] ? 0 : f[2];
+  }
+  return p;
+}
+
+inline PageTable page_table(const b200na_kv_cache& c, const int* table, int64_t stride, int max_pages) {
+  PageTable t{table, stride, max_pages, c.page_size, -1, c.pages};
+  for (int i = 0; i < 31; ++i)
+    if (c.page_size == 1 << i) t.shift = i;
+  return t;
+}
+
+inline int check_cache(const b200na_kv_cache* c, const int* table, int64_t table_stride, int max_pages,
+                       int dtype, int B) {
+  if (!c || c->pages < 0 || c->pages > 0x7fffffff || c->page_size < 1 || c->heads < 1 || c->head_dim < 1 ||
+      max_pages < 0 || B < 0 || (B > 1 && table_stride < 0))
+    return B200NA_ERR_INVALID_ARGUMENT;
+  if (c->head_dim > 256) return B200NA_ERR_UNSUPPORTED;
+  if (dtype != B200NA_F32 && dtype != B200NA_F16 && dtype != B200NA_BF16) return B200NA_ERR_UNSUPPORTED;
+  if (c->dtype == B200NA_E4M3) {
+    if (c->pages > 0 && (!c->key_scale || !c->value_scale)) return B200NA_ERR_INVALID_ARGUMENT;
+  } else if (c->dtype != dtype) {
+    return B200NA_ERR_INVALID_ARGUMENT;
+  }
+  if (c->pages > 0 && (!c->key || !c->value)) return B200NA_ERR_INVALID_ARGUMENT;
+  if (B > 0 && max_pages > 0 && !table) return B200NA_ERR_INVALID_ARGUMENT;
+  return B200NA_OK;
+}
+
+// ---- elements -----------------------------------------------------------------------------------------
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_float(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __nv_fp8_e4m3 from_float<__nv_fp8_e4m3>(float v) {
+  return __nv_fp8_e4m3(v);
+}
+
+template <class T, int kN>
+struct alignas(sizeof(T) * kN) Elements {
+  T v[kN];
+};
+
+}  // namespace b200na

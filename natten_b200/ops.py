@@ -9,8 +9,8 @@ current stream and raises on a non-zero status. Argument validation lives in ``f
 
 ``NATTEN_B200_DISABLE_TORCH_OPS=1`` turns the registration off (the functions are then called
 directly), like the reference's ``NATTEN_DISABLE_TORCH_OPS`` (src/natten/utils/environment.py:67-69).
-Autograd formulas are registered for `na_forward` (functional.py) and `fmha_forward`; the other
-ops have none, so differentiating through them raises.
+Autograd formulas are registered for `na_forward` (functional.py), `fmha_forward` and `rotary`; the
+other ops have none, so differentiating through them raises.
 """
 import ctypes
 import math
@@ -40,12 +40,12 @@ def _flags(xs) -> List[int]:
     return [1 if x else 0 for x in xs]
 
 
-def _op(name: str, fake: Callable):
+def _op(name: str, fake: Callable, mutates: Tuple[str, ...] = ()):
     """Registers ``fn`` as ``natten_b200::<name>`` with ``fake`` as its shape/dtype twin."""
     def wrap(fn):
         if not USE_TORCH_OPS:
             return fn
-        op = torch.library.custom_op(f"{NAMESPACE}::{name}", fn, mutates_args=(),
+        op = torch.library.custom_op(f"{NAMESPACE}::{name}", fn, mutates_args=mutates,
                                      device_types="cuda")
         op.register_fake(fake)
         # the plain function, for callers that already run inside another op's body (a second
@@ -382,3 +382,152 @@ def _fmha_backward(ctx, d_out, d_lse):
 
 if USE_TORCH_OPS:
     fmha_forward.register_autograd(_fmha_backward, setup_context=_fmha_setup_context)
+
+
+# ---- rotary positions ------------------------------------------------------------------------------
+
+POSITION_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _rotary_fake(query, key, axis_dims, theta, position_scale, origin, positions, interleaved, inverse):
+    return (query.new_empty(query.shape),
+            query.new_empty((0,)) if key is None else key.new_empty(key.shape))
+
+
+@_op("rotary", _rotary_fake)
+def rotary(query: Tensor, key: Optional[Tensor], axis_dims: List[int], theta: List[float],
+           position_scale: List[float], origin: List[int], positions: Optional[Tensor],
+           interleaved: bool, inverse: bool) -> Tuple[Tensor, Tensor]:
+    """Turns the channel pairs of ``[B, *X, H, D]`` query and key (an empty tensor when there is none)
+    by their tokens' positions; `inverse` turns back. Any strides with contiguous channels."""
+    out = _rotary_fake(query, key, axis_dims, theta, position_scale, origin, positions, interleaved,
+                       inverse)
+    query, key = (t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+                  for t in (query, key))
+    if positions is not None:
+        positions = positions.contiguous()
+    if query.numel() == 0:
+        return out
+    na_dim = query.dim() - 3
+    with torch.cuda.device(query.device):
+        _lib.check(_lib.lib.b200na_rotary(
+            _ptr(query), _ptr(key), _ptr(out[0]), _ptr(out[1]), na_dim,
+            _lib.ints(query.shape[1:1 + na_dim]), query.shape[0], query.shape[-2],
+            0 if key is None else key.shape[-2], query.shape[-1], DTYPE_CODE[query.dtype],
+            _lib.longs(query.stride()[:-1]), None if key is None else _lib.longs(key.stride()[:-1]),
+            len(axis_dims), _lib.ints(axis_dims), _lib.doubles(theta), _lib.doubles(position_scale),
+            _lib.longs(origin), _ptr(positions),
+            0 if positions is None else POSITION_CODE[positions.dtype],
+            0 if positions is None or positions.shape[0] == 1 else 1, int(interleaved), int(inverse),
+            _stream(query)), "b200na_rotary")
+    return out
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    _, key, *ctx.how, positions, ctx.interleaved, ctx.inverse = inputs
+    ctx.has_key = key is not None
+    ctx.save_for_backward(positions)
+
+
+def _rotary_backward(ctx, d_query, d_key):
+    # the transpose of a rotation: turn the gradients back (by the same op, so they can be
+    # differentiated again)
+    positions, = ctx.saved_tensors
+    more = (*ctx.how, positions, ctx.interleaved, not ctx.inverse)
+    need_q, need_k = ctx.needs_input_grad[0], ctx.has_key and ctx.needs_input_grad[1]
+    if need_q:
+        d_query, d_key = rotary(d_query, d_key if need_k else None, *more)
+    elif need_k:
+        d_key = rotary(d_key, None, *more)[0]
+    return (d_query if need_q else None, d_key if need_k else None, *[None] * 7)
+
+
+if USE_TORCH_OPS:
+    rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup_context)
+
+
+# ---- paged key/value cache ---------------------------------------------------------------------------
+
+def _cache_struct(key_pages: Tensor, value_pages: Tensor, key_scales: Optional[Tensor],
+                  value_scales: Optional[Tensor]) -> "_lib.KvCacheStruct":
+    c = _lib.KvCacheStruct()
+    c.key, c.value = key_pages.data_ptr(), value_pages.data_ptr()
+    c.key_stride[:], c.value_stride[:] = key_pages.stride()[:3], value_pages.stride()[:3]
+    if key_scales is not None:
+        c.key_scale, c.value_scale = key_scales.data_ptr(), value_scales.data_ptr()
+        c.key_scale_stride[:], c.value_scale_stride[:] = key_scales.stride(), value_scales.stride()
+    c.pages, c.page_size, c.heads, c.head_dim = key_pages.shape
+    c.dtype = DTYPE_CODE[key_pages.dtype]
+    return c
+
+
+def _kv_cache_write_fake(key, value, key_pages, value_pages, key_scales, value_scales, table, start,
+                         counts):
+    return None
+
+
+@_op("kv_cache_write", _kv_cache_write_fake,
+     mutates=("key_pages", "value_pages", "key_scales", "value_scales"))
+def kv_cache_write(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor,
+                   key_scales: Optional[Tensor], value_scales: Optional[Tensor], table: Tensor,
+                   start: Optional[Tensor], counts: Optional[Tensor]) -> None:
+    """Puts ``[B, T, Hkv, D]`` keys and values into the pages that `table` names."""
+    key, value = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (key, value))
+    cache = _cache_struct(key_pages, value_pages, key_scales, value_scales)
+    with torch.cuda.device(key.device):
+        _lib.check(_lib.lib.b200na_kv_cache_write(
+            ctypes.byref(cache), _ptr(key), _ptr(value), key.shape[0], key.shape[1],
+            DTYPE_CODE[key.dtype], _lib.longs(key.stride()[:3]), _lib.longs(value.stride()[:3]),
+            _ptr(table), table.stride(0), table.shape[1], _ptr(start), _ptr(counts), _stream(key)),
+            "b200na_kv_cache_write")
+
+
+def _kv_cache_read_fake(key_pages, value_pages, key_scales, value_scales, table, start, counts, length,
+                        dtype):
+    shape = (table.shape[0], length, *key_pages.shape[2:])
+    return tuple(key_pages.new_empty(shape, dtype=dtype) for _ in range(2))
+
+
+@_op("kv_cache_read", _kv_cache_read_fake)
+def kv_cache_read(key_pages: Tensor, value_pages: Tensor, key_scales: Optional[Tensor],
+                  value_scales: Optional[Tensor], table: Tensor, start: Optional[Tensor],
+                  counts: Optional[Tensor], length: int, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    """Contiguous ``[B, length, Hkv, D]`` keys and values out of the pages that `table` names."""
+    key, value = _kv_cache_read_fake(key_pages, value_pages, key_scales, value_scales, table, start,
+                                     counts, length, dtype)
+    cache = _cache_struct(key_pages, value_pages, key_scales, value_scales)
+    with torch.cuda.device(table.device):
+        _lib.check(_lib.lib.b200na_kv_cache_read(
+            ctypes.byref(cache), _ptr(key), _ptr(value), table.shape[0], length, DTYPE_CODE[dtype],
+            _ptr(table), table.stride(0), table.shape[1], _ptr(start), _ptr(counts), _stream(table)),
+            "b200na_kv_cache_read")
+    return key, value
+
+
+def _na1d_decode_fake(query, key_pages, value_pages, key_scales, value_scales, table, lengths,
+                      kernel_size, dilation, scale):
+    return _attn_fake(query)
+
+
+@_op("na1d_decode", _na1d_decode_fake)
+def na1d_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, key_scales: Optional[Tensor],
+                value_scales: Optional[Tensor], table: Tensor, lengths: Tensor, kernel_size: int,
+                dilation: int, scale: float) -> Tuple[Tensor, Tensor]:
+    """Attention of ``[B, T, Hq, D]`` newest tokens over the pages that `table` names."""
+    if query.stride(-1) != 1 and query.shape[-1] != 1:
+        query = query.contiguous()
+    out, lse = _attn_fake(query)
+    cache = _cache_struct(key_pages, value_pages, key_scales, value_scales)
+    B, T, Hq, _ = query.shape
+    dt = DTYPE_CODE[query.dtype]
+    with torch.cuda.device(query.device):
+        need = _lib.lib.b200na_na1d_decode_workspace(B, T, Hq, ctypes.byref(cache), table.shape[1],
+                                                     kernel_size, dilation, dt)
+        if need < 0:
+            _lib.check(int(need), "b200na_na1d_decode_workspace", kernel_launches=0)
+        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        _lib.check(_lib.lib.b200na_na1d_decode(
+            _ptr(query), _lib.longs(query.stride()[:3]), ctypes.byref(cache), _ptr(out), _ptr(lse), B, T,
+            Hq, dt, _ptr(table), table.stride(0), table.shape[1], _ptr(lengths), kernel_size, dilation,
+            float(scale), _ptr(workspace), _stream(query)), "b200na_na1d_decode", kernel_launches=2)
+    return out, lse
