@@ -8,7 +8,7 @@
 // counts is that all SMs read all the time, whatever the sequences' lengths are.
 //
 // Work: an item is one sequence, one key/value head and up to 16 (CUDA cores: 8) rows, which are the heads
-// of the group times neighbouring query tokens. Its keys are cut into units of 64. The units of all items
+// of the group times neighbouring query tokens. Its keys are cut into units of 64 or 128. The units of all items
 // in a row are cut into as many equal ranges as there are blocks; lengths are read on the device, so the
 // host waits for nothing and a captured launch follows them. A block keeps the running maximum and sum of
 // each row over its range of an item and either writes the result (it had the whole item) or leaves a part
@@ -21,7 +21,6 @@ namespace b200na {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kUnit = 64;             // keys of a unit of work
 constexpr int kMostParts = 2 * 148;   // blocks of the first launch: two per SM
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -42,6 +41,7 @@ struct DecodeArgs {
   int token_blocks, head_blocks;
   int64_t items;                      // of one sequence
   int parts;
+  int unit;                           // keys of a unit of work: a tile for each warp of a block
   int2* covered;                      // [B * items]: first block that worked on the item, how many
   float2* part_ml;                    // [2 * parts][rows]: maximum (of scale_log2 * q.k) and sum
   float* part_o;                      // [2 * parts][rows][D]
@@ -54,7 +54,7 @@ __device__ __forceinline__ int64_t units_of(const DecodeArgs& a, int length) {
   const int64_t widest = a.window + (a.dilation > 1 ? 0 : a.item_tokens - 1);
   n = n < a.capacity ? n : a.capacity;
   n = n < widest ? n : widest;
-  return n > 0 ? (n + kUnit - 1) / kUnit : 1;   // an item without keys still has its rows written
+  return n > 0 ? (n + a.unit - 1) / a.unit : 1;   // an item without keys still has its rows written
 }
 
 struct Item {
@@ -178,10 +178,10 @@ __device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, int6
 }
 
 // Merges the warps' maxima, sums and outputs of the item's rows and writes them out. `o` holds the warps'
-// unnormalised outputs [kWarps][rows_max][D], ml their (maximum, sum) [kWarps][rows_max].
+// unnormalised outputs [kWarps][rows_max][o_stride], ml their (maximum, sum) [kWarps][rows_max].
 template <class T>
 __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int part, const float* o,
-                                      const float2* ml, int rows_max) {
+                                      int o_stride, const float2* ml, int rows_max) {
   const int rows = it.tokens * it.heads;
   for (int i = threadIdx.x; i < rows * a.D; i += kThreads) {
     const int row = i / a.D, d = i - row * a.D;
@@ -194,7 +194,7 @@ __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int p
       if (p.x == -INFINITY) continue;         // the warp met no key of this row
       const float f = exp2f(p.x - m);
       l += f * p.y;
-      x += f * o[(w * rows_max + row) * a.D + d];
+      x += f * o[(w * rows_max + row) * o_stride + d];
     }
     if (part < 0) {
       const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 #pragma unroll
       for (int e = 0; e < kD32; ++e) acc[x][e] = 0.f;
     }
-    const int64_t begin = (at - item_begin) * kUnit;
-    const int64_t end = min((stop - item_begin) * kUnit, it.n);
+    const int64_t begin = (at - item_begin) * a.unit;
+    const int64_t end = min((stop - item_begin) * a.unit, it.n);
     for (int64_t i0 = begin + warp * 32; i0 < end; i0 += kWarps * 32) {
       const int64_t i = i0 + lane, j = it.first + i * a.dilation;
       int64_t page = -1;
@@ -341,7 +341,452 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
-    leave<T>(a, it, part, o, ml, kRows);
+    leave<T>(a, it, part, o, a.D, ml, kRows);
+    at = stop;
+  }
+}
+
+// ---- tensor cores: fp16 / bf16 queries, 16-byte rows ---------------------------------------------------
+// A warp works alone on tiles of kKeys keys with copies of its own (cp.async, kStages tiles in flight), so
+// nothing waits for another warp before the item's end: 128 KB in flight per SM. The products are small next
+// to the bytes (16 rows are padded to the instruction's 16, 2 x 16 flops a cached element), so mma.sync on
+// fragments that ldmatrix takes out of the copied rows is enough; tcgen05 would want 128-row tiles and the
+// probabilities in shared memory or TMEM for the same bytes.
+//
+// 8-bit rows are converted to fp16, which holds every e4m3 value, in registers. A key's scale multiplies its
+// logits; a value's scale goes into its weight as 2^(s_j + log2 scale_j - m'), with a running maximum m' of
+// its own, so that the largest of these weights is 1 whatever the scales are and fp16 loses only what is
+// 2^-24 of it. Queries are multiplied by a power of two that brings the row's largest to [1, 2), exactly.
+template <class T> struct Half2Of;
+template <> struct Half2Of<__half> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Half2Of<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+template <bool kTrans> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  if (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+template <class M> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (std::is_same<M, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two e4m3 values (low 16 bits) -> two fp16 values
+__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t x) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int kDP, bool k8> struct Tile {
+  static constexpr int kRowBytes = kDP * (k8 ? 1 : 2);
+  static constexpr int kChunks = kRowBytes / 16;                   // of a row
+  static constexpr int kKeys = kRowBytes >= 256 ? 16 : 32;
+  static constexpr int kStages = 3;
+  static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
+  static constexpr int kExtra = 16 + (k8 ? 2 * kKeys * 4 : 0);     // which keys are there; scales
+  static constexpr int kStage = 2 * kMatrix + kExtra;
+  static constexpr int kRows = 16;
+  static size_t bytes(int D) {
+    const size_t tiles = (size_t)kWarps * kStages * kStage, merge = (size_t)kWarps * kRows * (D + 8) * sizeof(float);
+    return tiles > merge ? tiles : merge;
+  }
+  // Chunks of a row are permuted so that eight neighbouring rows have any one chunk in eight different
+  // groups of banks.
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
+    const int x = kChunks >= 8 ? row & 7 : kChunks == 4 ? row >> 1 & 3 : row >> 2 & 1;
+    return row * kRowBytes + ((chunk ^ x) << 4);
+  }
+};
+
+template <class T, bool k8, int kDP>
+__global__ void __launch_bounds__(kThreads, kDP == 256 && !k8 ? 1 : 2)
+decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
+  using M = typename std::conditional<k8, __half, T>::type;        // operands of the products
+  using L = Tile<kDP, k8>;
+  constexpr int kKeys = L::kKeys, kStages = L::kStages, kGroups = kKeys / 16, kSteps = kDP / 16;
+  extern __shared__ __align__(128) uint8_t tiles[];
+  __shared__ float2 ml[kWarps * 16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = lane >> 2, c = lane & 3;                          // rows r0, r0 + 8 and columns 2c, 2c + 1
+  uint8_t* const mine = tiles + warp * kStages * L::kStage;
+  const uint32_t mine_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+  constexpr int kElem = k8 ? 1 : 2;
+  const int real_chunks = a.D * kElem / 16;
+
+  const Range r = my_range(a);
+  int b = r.b;
+  int64_t before = r.before;
+  for (int64_t at = r.begin; at < r.end;) {
+    const int length = a.lengths[b];
+    const int64_t units = units_of(a, length);
+    const int64_t index = (at - before) / units;
+    if (index >= a.items) {
+      before += units * a.items;
+      ++b;
+      continue;
+    }
+    const Item it = item_of(a, b, index, length);
+    const int64_t item_begin = before + index * units, item_end = item_begin + units;
+    const int64_t stop = item_end < r.end ? item_end : r.end;
+    const int rows = it.tokens * it.heads;
+    const int64_t begin = (at - item_begin) * a.unit + warp * kKeys;
+    const int64_t end = min((stop - item_begin) * a.unit, it.n);
+    const int count = end > begin ? (int)((end - begin + a.unit - 1) / a.unit) : 0;   // of this warp's tiles
+
+    // the table's entry for this lane's key of tile `s`
+    const auto entry = [&](int s, int64_t* page, int* slot) {
+      const int64_t i = begin + (int64_t)s * a.unit + (lane & (kKeys - 1));
+      *page = -1;
+      *slot = 0;
+      if (s < count && i < end) {
+        int64_t pi;
+        a.table.split(it.first + i * a.dilation, &pi, slot);
+        *page = a.table.page_of(b, pi);
+      }
+    };
+    const auto fetch = [&](int s, int64_t page, int slot) {
+      const uint32_t base = mine_u32 + (s % kStages) * L::kStage;
+      const bool there = page >= 0;
+      int64_t k_at = -1, v_at = -1;
+      if (there) {
+        k_at = page * a.key.page + (int64_t)slot * a.key.token + it.head * a.key.head;
+        v_at = page * a.value.page + (int64_t)slot * a.value.token + it.head * a.value.head;
+      }
+      if (s < count) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(mine + (s % kStages) * L::kStage + 2 * L::kMatrix) = mask;
+        constexpr int kRowsAtOnce = 32 / L::kChunks;
+        const int chunk = lane % L::kChunks;
+#pragma unroll
+        for (int i = 0; i < kKeys / kRowsAtOnce; ++i) {
+          const int row = i * kRowsAtOnce + lane / L::kChunks;
+          const int64_t ka = __shfl_sync(0xffffffffu, k_at, row), va = __shfl_sync(0xffffffffu, v_at, row);
+          const bool ok = ka >= 0 && chunk < real_chunks;          // zeros elsewhere
+          const uint8_t* k = static_cast<const uint8_t*>(a.key.base) + (ok ? ka * kElem + chunk * 16 : 0);
+          const uint8_t* v = static_cast<const uint8_t*>(a.value.base) + (ok ? va * kElem + chunk * 16 : 0);
+          copy16(base + L::at(row, chunk), k, ok);
+          copy16(base + L::kMatrix + L::at(row, chunk), v, ok);
+        }
+        if (k8 && lane < kKeys) {
+          const int64_t ks = there ? page * a.key.s_page + (int64_t)slot * a.key.s_token + it.head * a.key.s_head : 0;
+          const int64_t vs = there ? page * a.value.s_page + (int64_t)slot * a.value.s_token + it.head * a.value.s_head : 0;
+          copy4(base + 2 * L::kMatrix + 16 + lane * 4, a.key.scale + ks, there);
+          copy4(base + 2 * L::kMatrix + 16 + (kKeys + lane) * 4, a.value.scale + vs, there);
+        }
+      }
+      copy_commit();
+    };
+    int64_t page;
+    int slot;
+    entry(0, &page, &slot);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      fetch(s, page, slot);
+      entry(s + 1, &page, &slot);
+    }
+
+    // The queries as A fragments: rows r0 and r0 + 8. 16-bit caches: channels 16 k + 2c, + 1 and 8 further;
+    // 8-bit ones: 16 k + 4c .. + 3, the four that one 32-bit word of a key row holds.
+    uint32_t q[kSteps][4];
+    float row_scale[2];
+    int row_token[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = r0 + 8 * x;
+      row_token[x] = row / it.heads;
+      const T* src = nullptr;
+      if (row < rows) {
+        const int t = it.t0 + row_token[x], h = it.head * a.group + it.h0 + row % it.heads;
+        src = static_cast<const T*>(a.query) + b * a.q_batch + t * a.q_token + h * a.q_head;
+      }
+      T v[kSteps][4];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 16 * k + (k8 ? 4 * c + e : 2 * c + (e & 1) + 8 * (e >> 1));
+          v[k][e] = src && d < a.D ? src[d] : from_float<T>(0.f);
+        }
+      float factor = 1.f;
+      row_scale[x] = a.scale_log2;
+      if (k8) {
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(as_float(v[k][e])));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // 2^-e and 2^e of the largest magnitude's exponent, where both are normal numbers
+        const int e = (__float_as_int(most) >> 23) - 127;
+        if (e > -126 && e < 127) {
+          factor = __int_as_float((127 - e) << 23);
+          row_scale[x] *= __int_as_float((127 + e) << 23);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          q[k][x + 2 * e] = Half2Of<M>::pack(as_float(v[k][2 * e]) * factor, as_float(v[k][2 * e + 1]) * factor);
+    }
+
+    float acc[kDP / 8][4], m[2], l[2], mv[2];
+#pragma unroll
+    for (int i = 0; i < kDP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      m[x] = mv[x] = -INFINITY;
+      l[x] = 0.f;
+    }
+
+    for (int s = 0; s < count; ++s) {
+      copy_wait<kStages - 2>();
+      __syncwarp();                        // the tile is there, and everyone is done with the one before it
+      fetch(s + kStages - 1, page, slot);
+      entry(s + kStages, &page, &slot);
+      const uint32_t base = mine_u32 + (s % kStages) * L::kStage;
+      const uint8_t* extra = mine + (s % kStages) * L::kStage + 2 * L::kMatrix;
+      uint32_t there = *reinterpret_cast<const uint32_t*>(extra);
+      if (kKeys < 32) there &= (1u << (kKeys & 31)) - 1;
+
+      float p[2 * kGroups][4];
+#pragma unroll
+      for (int i = 0; i < 2 * kGroups; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[i][e] = 0.f;
+      if constexpr (!k8) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            uint32_t f[4];
+            ldmatrix4<false>(f, base + L::at(16 * g + (lane & 7) + (lane >> 4) * 8, 2 * k + (lane >> 3 & 1)));
+            mma<M>(p[2 * g], q[k], f[0], f[1]);
+            mma<M>(p[2 * g + 1], q[k], f[2], f[3]);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; k += 2)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            uint32_t f[4];
+            ldmatrix4<false>(f, base + L::at(16 * g + (lane & 15), k + (lane >> 4)));
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              mma<M>(p[2 * g], q[k + z], e4m3_to_f16(f[2 * z]), e4m3_to_f16(f[2 * z] >> 16));
+              mma<M>(p[2 * g + 1], q[k + z], e4m3_to_f16(f[2 * z + 1]), e4m3_to_f16(f[2 * z + 1] >> 16));
+            }
+          }
+      }
+
+      // which keys each row attends
+      const int64_t i0 = begin + (int64_t)s * a.unit;
+      const int64_t j0 = it.first + i0 * a.dilation;
+      const bool differ = it.tokens > 1 && !(j0 + kKeys - 1 <= it.p0 && j0 > it.p0 + it.tokens - 1 - a.window);
+      constexpr uint32_t kAll = kKeys < 32 ? (1u << (kKeys & 31)) - 1 : 0xffffffffu;
+      uint32_t on[2] = {there, there};
+      if (differ) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          // keys j <= p: the first p - j0 + 1; keys j > p - window: not the first p - window - j0 + 1
+          const int64_t pos = it.p0 + row_token[x] - j0;
+          const int64_t upto = pos + 1, from = pos - a.window + 1;
+          on[x] &= upto <= 0 ? 0u : upto >= 32 ? 0xffffffffu : (1u << (int)upto) - 1;
+          on[x] &= from <= 0 ? 0xffffffffu : from >= 32 ? 0u : ~((1u << (int)from) - 1);
+        }
+      }
+      const float* k_scale = reinterpret_cast<const float*>(extra + 16);
+      const float* v_scale = k_scale + kKeys;
+      float top[2] = {-INFINITY, -INFINITY}, lv[2 * kGroups][2];
+#pragma unroll
+      for (int i = 0; i < 2 * kGroups; ++i) {
+        float2 ks = make_float2(1.f, 1.f);
+        if (k8) {
+          ks = *reinterpret_cast<const float2*>(k_scale + 8 * i + 2 * c);
+          const float2 vs = *reinterpret_cast<const float2*>(v_scale + 8 * i + 2 * c);
+          lv[i][0] = __log2f(vs.x);
+          lv[i][1] = __log2f(vs.y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[i][e] *= k8 ? row_scale[e >> 1] * (e & 1 ? ks.y : ks.x) : row_scale[e >> 1];
+          if (on[e >> 1] != kAll && !(on[e >> 1] >> (8 * i + 2 * c + (e & 1)) & 1)) p[i][e] = -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], p[i][e]);
+        }
+      }
+      float topv[2] = {-INFINITY, -INFINITY};
+      if (k8) {
+#pragma unroll
+        for (int i = 0; i < 2 * kGroups; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) topv[e >> 1] = fmaxf(topv[e >> 1], p[i][e] + lv[i][e & 1]);
+      }
+      float base_m[2], base_v[2], keep[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+        const float next = fmaxf(m[x], top[x]);
+        // nothing attended yet: no difference of infinities. (A NaN logit is passed over by the maximum and
+        // comes back in the exponential.)
+        base_m[x] = next == -INFINITY ? 0.f : next;
+        keep[x] = ex2(m[x] - base_m[x]);
+        l[x] *= keep[x];
+        m[x] = next;
+        if (k8) {
+          topv[x] = fmaxf(topv[x], __shfl_xor_sync(0xffffffffu, topv[x], 1));
+          topv[x] = fmaxf(topv[x], __shfl_xor_sync(0xffffffffu, topv[x], 2));
+          const float nextv = fmaxf(mv[x], topv[x]);
+          base_v[x] = nextv == -INFINITY ? 0.f : nextv;
+          keep[x] = ex2(mv[x] - base_v[x]);
+          mv[x] = nextv;
+        }
+      }
+      if (keep[0] != 1.f || keep[1] != 1.f) {
+#pragma unroll
+        for (int i = 0; i < kDP / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][e] *= keep[e >> 1];
+      }
+      uint32_t w[kGroups][4];              // the weights as A fragments
+#pragma unroll
+      for (int i = 0; i < 2 * kGroups; ++i) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = p[i][e];
+          const float ex = ex2(x - base_m[e >> 1]);
+          l[e >> 1] += ex;
+          y[e] = k8 ? ex2(x + lv[i][e & 1] - base_v[e >> 1]) : ex;
+          // a token left out has the scale 0 or any other: its weight is 0
+          if (k8 && x == -INFINITY) y[e] = 0.f;
+        }
+        w[i >> 1][2 * (i & 1)] = Half2Of<M>::pack(y[0], y[1]);
+        w[i >> 1][2 * (i & 1) + 1] = Half2Of<M>::pack(y[2], y[3]);
+      }
+
+      // values: B fragments of two (8-bit: four) 8-channel columns for 16 keys at a time
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const auto column = [&](int n, uint32_t b0, uint32_t b1) {
+          if (!differ) {
+            mma<M>(acc[n], w[g], b0, b1);
+          } else {
+            // Rows attend different keys of this tile: a NaN or an infinity of a value must stay with the
+            // rows that attend it, so every query token gets the values with the others' taken out.
+            for (int t = 0; t < it.tokens; ++t) {
+              const int64_t pos = it.p0 + t - j0;
+              const int64_t upto = pos + 1, from = pos - a.window + 1;
+              uint32_t seen = there;
+              seen &= upto <= 0 ? 0u : upto >= 32 ? 0xffffffffu : (1u << (int)upto) - 1;
+              seen &= from <= 0 ? 0xffffffffu : from >= 32 ? 0u : ~((1u << (int)from) - 1);
+              seen >>= 16 * g + 2 * c;
+              const uint32_t s0 = (seen & 1 ? 0xffffu : 0u) | (seen & 2 ? 0xffff0000u : 0u);
+              const uint32_t s1 = (seen >> 8 & 1 ? 0xffffu : 0u) | (seen >> 8 & 2 ? 0xffff0000u : 0u);
+              float part[4] = {0.f, 0.f, 0.f, 0.f};
+              mma<M>(part, w[g], b0 & s0, b1 & s1);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (row_token[e >> 1] == t) acc[n][e] += part[e];
+            }
+          }
+        };
+        if constexpr (!k8) {
+#pragma unroll
+          for (int n = 0; n < kSteps; ++n) {
+            uint32_t f[4];
+            ldmatrix4<true>(f, base + L::kMatrix + L::at(16 * g + (lane & 15), 2 * n + (lane >> 4)));
+            column(2 * n, f[0], f[1]);
+            column(2 * n + 1, f[2], f[3]);
+          }
+        } else {
+          // a 16-bit unit holds channels d, d + 1 of a key: sorted into pairs of keys for d and for d + 1
+#pragma unroll
+          for (int n = 0; n < kSteps; n += 2) {
+            uint32_t f[4];
+            ldmatrix4<true>(f, base + L::kMatrix + L::at(16 * g + (lane & 15), n + (lane >> 4)));
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t lo = f[2 * z], hi = f[2 * z + 1];
+              column(2 * (n + z), e4m3_to_f16(__byte_perm(lo, 0, 0x4420)), e4m3_to_f16(__byte_perm(hi, 0, 0x4420)));
+              column(2 * (n + z) + 1, e4m3_to_f16(__byte_perm(lo, 0, 0x4431)), e4m3_to_f16(__byte_perm(hi, 0, 0x4431)));
+            }
+          }
+        }
+      }
+    }
+
+    // the warps' results side by side in shared memory
+    copy_wait<0>();
+    __syncthreads();
+    float* const o = reinterpret_cast<float*>(tiles);
+    const int o_stride = a.D + 8;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      if (m[x] == -INFINITY && l[x] != l[x]) m[x] = 0.f;           // only NaN logits: they count
+      const int row = r0 + 8 * x;
+      if (row >= rows) continue;
+      if (c == 0) ml[warp * 16 + row] = make_float2(m[x], l[x]);
+      if (m[x] == -INFINITY) continue;                             // (not read)
+      const float f = k8 ? ex2(mv[x] - m[x]) : 1.f;
+      float* const dst = o + (warp * 16 + row) * o_stride;
+      if constexpr (!k8) {
+#pragma unroll
+        for (int i = 0; i < kDP / 8; ++i)
+          if (8 * i + 2 * c < a.D)
+            *reinterpret_cast<float2*>(dst + 8 * i + 2 * c) = make_float2(acc[i][2 * x], acc[i][2 * x + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+          if (16 * i + 4 * c < a.D)
+            *reinterpret_cast<float4*>(dst + 16 * i + 4 * c) =
+                make_float4(f * acc[2 * i][2 * x], f * acc[2 * i + 1][2 * x], f * acc[2 * i][2 * x + 1],
+                            f * acc[2 * i + 1][2 * x + 1]);
+      }
+    }
+    __syncthreads();
+    const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
+    leave<T>(a, it, part, o, o_stride, ml, 16);
+    __syncthreads();                                               // before the next item's tiles come
     at = stop;
   }
 }
@@ -393,11 +838,24 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
 // ---- host --------------------------------------------------------------------------------------------------
 
 struct Plan {
+  bool tensor_cores;
   int rows_max;             // rows of an item
+  int unit;
   int item_tokens, item_heads, token_blocks, head_blocks, parts;
   int64_t items;
   int64_t covered_bytes, ml_bytes, o_bytes;
 };
+
+// Whether the tensor-core kernel reads this cache: rows of whole 16-byte pieces on 16-byte boundaries, for
+// 16-bit queries.
+bool reads_in_chunks(const b200na_kv_cache& c, int dtype) {
+  if (dtype != B200NA_F16 && dtype != B200NA_BF16) return false;
+  const int per = c.dtype == B200NA_E4M3 ? 16 : 8;
+  const PagedPool k = paged_pool(c, false), v = paged_pool(c, true);
+  return c.head_dim % per == 0 &&
+         (reinterpret_cast<uintptr_t>(c.key) | reinterpret_cast<uintptr_t>(c.value)) % 16 == 0 &&
+         (k.page | k.token | k.head | v.page | v.token | v.head) % per == 0;
+}
 
 int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -407,8 +865,11 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   if (rc != B200NA_OK) return rc;
   if (T < 0 || Hq < 1 || Hq % cache->heads || Hq > 65536 || kernel < 0 || dilation < 1)
     return B200NA_ERR_INVALID_ARGUMENT;
-  const int group = Hq / cache->heads;
-  p->rows_max = group == 1 && (T <= 1 || dilation > 1) ? 1 : 8;
+  const int group = Hq / cache->heads, D = cache->head_dim;
+  p->tensor_cores = reads_in_chunks(*cache, dtype);
+  p->rows_max = p->tensor_cores ? 16 : group == 1 && (T <= 1 || dilation > 1) ? 1 : 8;
+  // a tile for each of a block's warps
+  p->unit = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
   p->item_heads = group < p->rows_max ? group : p->rows_max;
   p->head_blocks = (group + p->item_heads - 1) / p->item_heads;
   p->item_tokens = dilation > 1 ? 1 : p->rows_max / p->item_heads;
@@ -419,8 +880,8 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   // units if every sequence were as long as the table allows
   int64_t most = (int64_t)max_pages * cache->page_size;
   if (kernel > 0 && most > (int64_t)kernel + p->item_tokens) most = (int64_t)kernel + p->item_tokens;
-  const int64_t units = B * p->items * (most / kUnit + 1);
-  if (most / kUnit + 1 > ((int64_t)1 << 52) / (B * p->items + 1)) return B200NA_ERR_INVALID_ARGUMENT;
+  const int64_t units = B * p->items * (most / p->unit + 1);
+  if (most / p->unit + 1 > ((int64_t)1 << 52) / (B * p->items + 1)) return B200NA_ERR_INVALID_ARGUMENT;
   p->parts = (int)(units < kMostParts ? (units < 1 ? 1 : units) : kMostParts);
   p->covered_bytes = round_up(B * p->items * (int64_t)sizeof(int2));
   p->ml_bytes = round_up((int64_t)2 * p->parts * p->rows_max * sizeof(float2));
@@ -460,9 +921,31 @@ int run_simt(const DecodeArgs& a, int rows_max, cudaStream_t s) {
   return a.D <= 128 ? launch_simt<T, P, 8, 4, false>(a, s) : launch_simt<T, P, 8, 8, false>(a, s);
 }
 
+template <class T, bool k8, int kDP>
+int launch_mma(const DecodeArgs& a, cudaStream_t s) {
+  const size_t smem = Tile<kDP, k8>::bytes(a.D);
+  const int rc = opt_in(decode_mma_kernel<T, k8, kDP>, smem);
+  if (rc != B200NA_OK) return rc;
+  decode_mma_kernel<T, k8, kDP><<<a.parts, kThreads, smem, s>>>(a);
+  B200NA_CUDA_TRY(cudaGetLastError());
+  return B200NA_OK;
+}
 template <class T>
-int run(const DecodeArgs& a, int cache_dtype, int rows_max, cudaStream_t s) {
-  int rc = cache_dtype == B200NA_E4M3 ? run_simt<T, __nv_fp8_e4m3>(a, rows_max, s) : run_simt<T, T>(a, rows_max, s);
+int run_mma(const DecodeArgs& a, bool eight_bits, cudaStream_t s) {
+  if constexpr (!std::is_same<T, float>::value) {
+    if (eight_bits)
+      return a.D <= 64 ? launch_mma<T, true, 64>(a, s) : a.D <= 128 ? launch_mma<T, true, 128>(a, s)
+                                                                    : launch_mma<T, true, 256>(a, s);
+    return a.D <= 64 ? launch_mma<T, false, 64>(a, s) : a.D <= 128 ? launch_mma<T, false, 128>(a, s)
+                                                                   : launch_mma<T, false, 256>(a, s);
+  }
+  return B200NA_ERR_UNSUPPORTED;
+}
+
+template <class T>
+int run(const DecodeArgs& a, bool tensor_cores, int cache_dtype, int rows_max, cudaStream_t s) {
+  int rc = tensor_cores ? run_mma<T>(a, cache_dtype == B200NA_E4M3, s)
+           : cache_dtype == B200NA_E4M3 ? run_simt<T, __nv_fp8_e4m3>(a, rows_max, s) : run_simt<T, T>(a, rows_max, s);
   if (rc != B200NA_OK) return rc;
   // The join's blocks may take their places while the first launch's last ones run (they wait for its end
   // before they read anything).
@@ -534,14 +1017,15 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.head_blocks = p.head_blocks;
   a.items = p.items;
   a.parts = p.parts;
+  a.unit = p.unit;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.covered = reinterpret_cast<int2*>(w);
   a.part_ml = reinterpret_cast<float2*>(w + p.covered_bytes);
   a.part_o = reinterpret_cast<float*>(w + p.covered_bytes + p.ml_bytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case B200NA_F32: return run<float>(a, cache->dtype, p.rows_max, s);
-    case B200NA_F16: return run<__half>(a, cache->dtype, p.rows_max, s);
-    default: return run<__nv_bfloat16>(a, cache->dtype, p.rows_max, s);
+    case B200NA_F32: return run<float>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
+    case B200NA_F16: return run<__half>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
+    default: return run<__nv_bfloat16>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
   }
 }
