@@ -495,7 +495,7 @@ B200NA_API int b200na_kv_cache_read(const b200na_kv_cache* cache, void* key, voi
  * nothing (p < 0, or no page) gives zeros and a logsumexp of -inf.
  * query: [B, T, Hq, D] of `dtype` fp32 / fp16 / bf16, element strides of batch, token and head; Hq a
  * multiple of the cache's heads; the cache's dtype is the query's, or B200NA_E4M3. out: contiguous
- * [B, T, Hq, D]; lse: NULL or contiguous fp32 [B, T, Hq]. workspace:
+ * [B, T, Hq, D], 16-byte aligned; lse: NULL or contiguous fp32 [B, T, Hq]. workspace:
  * b200na_na1d_decode_workspace(...) bytes, 16-byte aligned, for this call alone while it runs. Two
  * launches: parts of equal work whatever the lengths are, and their join.
  */

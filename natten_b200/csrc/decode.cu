@@ -27,127 +27,158 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct DecodeArgs {
   const void* query;
   int64_t q_batch, q_token, q_head;
+  bool q_words;                       // 16-bit queries: every pair of channels lies on 4 bytes
   void* out;
   float* lse;
   PagedPool key, value;
+  bool same_strides;                  // of the pools of keys and values
   PageTable table;
   const int* lengths;
-  int64_t capacity;                   // tokens that a row of the table can name
+  int capacity;                       // tokens that a row of the table can name
   int B, T, Hq, heads, group, D;      // heads: of keys and values; group: query heads of each
   int64_t window;                     // tokens attended at most
   int dilation;
   float scale_log2;
   int item_tokens, item_heads;        // query tokens and heads of an item: its rows
   int token_blocks, head_blocks;
-  int64_t items;                      // of one sequence
+  uint32_t items;                     // of one sequence
   int parts;
-  int unit;                           // keys of a unit of work: a tile for each warp of a block
+  int step;                           // keys that the warps of a block take at once: a tile each
+  int unit;                           // keys of a unit of work, a multiple of `step`
   int2* covered;                      // [B * items]: first block that worked on the item, how many
   float2* part_ml;                    // [2 * parts][rows]: maximum (of scale_log2 * q.k) and sum
   float* part_o;                      // [2 * parts][rows][D]
 };
 
-// What the blocks of a launch agree on: the units of a sequence (the same for each of its items).
-__device__ __forceinline__ int64_t units_of(const DecodeArgs& a, int length) {
-  int64_t n = length < 0 ? 0 : length;
+// What the blocks of a launch agree on: the units of a sequence (the same for each of its items). (The host
+// has seen to it that the units of all items together fit 31 bits.)
+__device__ __forceinline__ uint32_t units_of(const DecodeArgs& a, int length) {
+  int n = length < 0 ? 0 : length;
   if (a.dilation > 1) n = n > 0 ? (n - 1) / a.dilation + 1 : 0;
   const int64_t widest = a.window + (a.dilation > 1 ? 0 : a.item_tokens - 1);
   n = n < a.capacity ? n : a.capacity;
-  n = n < widest ? n : widest;
-  return n > 0 ? (n + a.unit - 1) / a.unit : 1;   // an item without keys still has its rows written
+  n = n < widest ? n : (int)widest;
+  return n > 0 ? ((uint32_t)n + a.unit - 1) / a.unit : 1;   // an item without keys still has its rows written
 }
 
 struct Item {
-  int64_t index;         // among the sequence's
   int b, head, t0, tokens, h0, heads;
-  int64_t p0;            // position of token t0
-  int64_t first, n;      // keys at first + dilation * i, i < n
+  int p0;                // position of token t0
+  int first, n;          // keys at first + dilation * i, i < n
 };
 
-__device__ __forceinline__ Item item_of(const DecodeArgs& a, int b, int64_t index, int length) {
+// The rows of an item: they do not depend on the sequence's length.
+__device__ __forceinline__ Item rows_of(const DecodeArgs& a, int b, uint32_t index) {
   Item it;
-  it.index = index;
   it.b = b;
-  const int hb = (int)(index % a.head_blocks);
-  const int64_t rest = index / a.head_blocks;
-  const int tb = (int)(rest % a.token_blocks);
-  it.head = (int)(rest / a.token_blocks);
+  uint32_t hb = 0, tb = 0, head = index;
+  if (a.head_blocks > 1) {
+    hb = head % a.head_blocks;
+    head /= a.head_blocks;
+  }
+  if (a.token_blocks > 1) {
+    tb = head % a.token_blocks;
+    head /= a.token_blocks;
+  }
+  it.head = head;
   it.t0 = tb * a.item_tokens;
   it.tokens = min(a.item_tokens, a.T - it.t0);
   it.h0 = hb * a.item_heads;
   it.heads = min(a.item_heads, a.group - it.h0);
-  const int64_t len = length < 0 ? 0 : length;
+  return it;
+}
+
+__device__ __forceinline__ Item item_of(const DecodeArgs& a, int b, uint32_t index, int length) {
+  Item it = rows_of(a, b, index);
+  const int len = length < 0 ? 0 : length;
   it.p0 = len - a.T + it.t0;
-  const int64_t last = it.p0 + it.tokens - 1;
+  const int last = it.p0 + it.tokens - 1;
   it.first = 0;
   it.n = 0;
   if (last < 0) return it;
   if (a.dilation > 1) {                       // one token an item
-    int64_t count = last / a.dilation + 1;
-    count = count < a.window ? count : a.window;
+    const int there = last / a.dilation + 1;
+    const int count = there < a.window ? there : (int)a.window;
     it.first = last - (count - 1) * a.dilation;
-    const int64_t there = it.first < a.capacity ? (a.capacity - 1 - it.first) / a.dilation + 1 : 0;
-    it.n = count < there ? count : there;
+    const int known = it.first < a.capacity ? (a.capacity - 1 - it.first) / a.dilation + 1 : 0;
+    it.n = count < known ? count : known;
   } else {
     const int64_t from = (it.p0 > 0 ? it.p0 : 0) - a.window + 1;
-    it.first = from > 0 ? from : 0;
-    const int64_t end = (last < a.capacity ? last : a.capacity - 1) + 1;
+    it.first = from > 0 ? (int)from : 0;
+    const int end = last < a.capacity ? last + 1 : a.capacity;
     it.n = end > it.first ? end - it.first : 0;
   }
   return it;
 }
 
-__device__ __forceinline__ int64_t range_begin(int64_t units, int part, int parts) {
-  return units * part / parts;
-}
+// The ranges of `parts` blocks over `total` units: equal to within one unit, the longer ones first.
+struct Split {
+  uint32_t base, extra;
+  __device__ __forceinline__ Split(uint32_t total, uint32_t parts) : base(total / parts), extra(total - base * parts) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t part) const { return part * base + min(part, extra); }
+  __device__ __forceinline__ uint32_t part_with(uint32_t unit) const {
+    const uint32_t longer = extra * (base + 1);
+    return unit < longer ? unit / (base + 1) : extra + (unit - longer) / base;
+  }
+};
 
 // The block's range of units and the sequence in which it begins. With fewer units than blocks the last
 // blocks have nothing to do: a block between an item's first and last one always has a unit of it.
 struct Range {
-  int64_t begin, end, total;
+  uint32_t begin, end, total;
   int parts;
-  int b;                 // sequence of `begin`
-  int64_t before;        // units of all sequences before it
+  int b, length;         // sequence of `begin`
+  uint32_t before;       // units of all sequences before it
 };
-__device__ Range my_range(const DecodeArgs& a) {
-  __shared__ int64_t sums[kWarps];
-  __shared__ int64_t found_before;
-  __shared__ int found_b;
+__device__ __forceinline__ Range my_range(const DecodeArgs& a) {
+  __shared__ uint32_t sums[kWarps];
+  __shared__ uint32_t found_before;
+  __shared__ int found_b, found_length;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t total = 0;
-  for (int b = threadIdx.x; b < a.B; b += kThreads) total += units_of(a, a.lengths[b]) * a.items;
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  // the first kThreads sequences, whose units are looked at again below
+  const int length0 = (int)threadIdx.x < a.B ? a.lengths[threadIdx.x] : 0;
+  const uint32_t units0 = (int)threadIdx.x < a.B ? units_of(a, length0) * a.items : 0;
+  uint32_t total = units0;
+  for (int b = threadIdx.x + kThreads; b < a.B; b += kThreads) total += units_of(a, a.lengths[b]) * a.items;
+  total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) sums[warp] = total;
   __syncthreads();
   Range r;
   r.total = 0;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) r.total += sums[w];
-  r.parts = (int)(r.total < a.parts ? r.total : a.parts);
-  r.begin = r.end = r.b = 0;
+  r.parts = (int)min(r.total, (uint32_t)a.parts);
+  r.begin = r.end = 0;
+  r.b = r.length = 0;
   r.before = 0;
   if ((int)blockIdx.x >= r.parts) return r;
-  r.begin = range_begin(r.total, blockIdx.x, r.parts);
-  r.end = range_begin(r.total, blockIdx.x + 1, r.parts);
-  int64_t before = 0;
+  const Split split(r.total, r.parts);
+  r.begin = split.begin(blockIdx.x);
+  r.end = split.begin(blockIdx.x + 1);
+  uint32_t before = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
     __syncthreads();
     const int b = b0 + threadIdx.x;
-    const int64_t mine = b < a.B ? units_of(a, a.lengths[b]) * a.items : 0;
-    int64_t incl = mine;
+    const int length = b0 == 0 ? length0 : b < a.B ? a.lengths[b] : 0;
+    const uint32_t mine = b0 == 0 ? units0 : b < a.B ? units_of(a, length) * a.items : 0;
+    uint32_t incl = mine;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
     }
     if (lane == 31) sums[warp] = incl;
     __syncthreads();
-    int64_t base = before, chunk = 0;
+    uint32_t base = before, chunk = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) base += sums[w];
       chunk += sums[w];
     }
-    const int64_t lo = base + incl - mine;
+    const uint32_t lo = base + incl - mine;
     if (lo <= r.begin && r.begin < lo + mine) {
       found_b = b;
+      found_length = length;
       found_before = lo;
     }
     before += chunk;
@@ -155,6 +186,7 @@ __device__ Range my_range(const DecodeArgs& a) {
   }
   __syncthreads();
   r.b = found_b;
+  r.length = found_length;
   r.before = found_before;
   return r;
 }
@@ -162,30 +194,26 @@ __device__ Range my_range(const DecodeArgs& a) {
 // How a segment (the block's part of an item) leaves: whole, or as part 0 (the item began in an earlier
 // block) or 1 of the block. The block that has the item's first unit notes which blocks the join has to
 // look at.
-__device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, int64_t item_begin,
-                                       int64_t item_end, int64_t item_id) {
-  if (item_begin >= r.begin && threadIdx.x == 0) {
-    int last = blockIdx.x;
-    if (item_end > r.end) {
-      last = (int)((item_end - 1) * r.parts / r.total);
-      while (range_begin(r.total, last + 1, r.parts) < item_end) ++last;
-      while (range_begin(r.total, last, r.parts) >= item_end) --last;
-    }
-    a.covered[item_id] = make_int2(blockIdx.x, last - blockIdx.x + 1);
-  }
-  if (item_begin >= r.begin && item_end <= r.end) return -1;
-  return item_begin < r.begin ? 0 : 1;
+__device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, uint32_t item_begin,
+                                       uint32_t item_end, int64_t item_id) {
+  const bool begins = item_begin >= r.begin, ends = item_end <= r.end;
+  if (begins && threadIdx.x == 0)
+    a.covered[item_id] = make_int2(
+        blockIdx.x, ends ? 1 : (int)Split(r.total, r.parts).part_with(item_end - 1) - (int)blockIdx.x + 1);
+  return begins && ends ? -1 : begins ? 1 : 0;
 }
 
 // Merges the warps' maxima, sums and outputs of the item's rows and writes them out. `o` holds the warps'
-// unnormalised outputs [kWarps][rows_max][o_stride], ml their (maximum, sum) [kWarps][rows_max].
-template <class T>
+// unnormalised outputs [kWarps][rows_max][o_stride], ml their (maximum, sum) [kWarps][rows_max]. kN channels
+// at a time.
+template <class T, int kN>
 __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int part, const float* o,
                                       int o_stride, const float2* ml, int rows_max) {
-  const int rows = it.tokens * it.heads;
-  for (int i = threadIdx.x; i < rows * a.D; i += kThreads) {
-    const int row = i / a.D, d = i - row * a.D;
-    float m = -INFINITY, l = 0.f, x = 0.f;
+  const int rows = it.tokens * it.heads, pieces = a.D / kN;
+  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
+    const int row = i / pieces, d = (i - row * pieces) * kN;
+    float m = -INFINITY, l = 0.f;
+    Elements<float, kN> x{};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * rows_max + row].x);
 #pragma unroll
@@ -194,16 +222,21 @@ __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int p
       if (p.x == -INFINITY) continue;         // the warp met no key of this row
       const float f = exp2f(p.x - m);
       l += f * p.y;
-      x += f * o[(w * rows_max + row) * o_stride + d];
+      const Elements<float, kN> y = *reinterpret_cast<const Elements<float, kN>*>(o + (w * rows_max + row) * o_stride + d);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
     }
     if (part < 0) {
       const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
       const int64_t at = ((int64_t)it.b * a.T + t) * a.Hq + h;
-      static_cast<T*>(a.out)[at * a.D + d] = from_float<T>(m == -INFINITY ? 0.f : x / l);
+      Elements<T, kN> y;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) y.v[e] = from_float<T>(m == -INFINITY ? 0.f : x.v[e] / l);
+      *reinterpret_cast<Elements<T, kN>*>(static_cast<T*>(a.out) + at * a.D + d) = y;
       if (d == 0 && a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
     } else {
       const int64_t slot = (int64_t)(2 * blockIdx.x + part) * rows_max + row;
-      a.part_o[slot * a.D + d] = x;
+      *reinterpret_cast<Elements<float, kN>*>(a.part_o + slot * a.D + d) = x;
       if (d == 0) a.part_ml[slot] = make_float2(m, l);
     }
   }
@@ -222,20 +255,18 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
   __shared__ float2 ml[kWarps * kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Range r = my_range(a);
-  int b = r.b;
-  int64_t before = r.before;
-  for (int64_t at = r.begin; at < r.end;) {
-    const int length = a.lengths[b];
-    const int64_t units = units_of(a, length);
-    const int64_t index = (at - before) / units;
+  int b = r.b, length = r.length;
+  uint32_t before = r.before;
+  for (uint32_t at = r.begin; at < r.end;) {
+    const uint32_t units = units_of(a, length), index = (at - before) / units;
     if (index >= a.items) {
       before += units * a.items;
-      ++b;
+      length = a.lengths[++b];
       continue;
     }
     const Item it = item_of(a, b, index, length);
-    const int64_t item_begin = before + index * units, item_end = item_begin + units;
-    const int64_t stop = item_end < r.end ? item_end : r.end;
+    const uint32_t item_begin = before + index * units, item_end = item_begin + units;
+    const uint32_t stop = min(item_end, r.end);
     const int rows = it.tokens * it.heads;
     __syncthreads();                                    // (the last segment's buffers are read)
     for (int i = threadIdx.x; i < kRows * a.D; i += kThreads) {
@@ -256,14 +287,15 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 #pragma unroll
       for (int e = 0; e < kD32; ++e) acc[x][e] = 0.f;
     }
-    const int64_t begin = (at - item_begin) * a.unit;
-    const int64_t end = min((stop - item_begin) * a.unit, it.n);
-    for (int64_t i0 = begin + warp * 32; i0 < end; i0 += kWarps * 32) {
-      const int64_t i = i0 + lane, j = it.first + i * a.dilation;
+    const int begin = (at - item_begin) * a.unit;
+    const int end = (int)min((int64_t)(stop - item_begin) * a.unit, (int64_t)it.n);
+    for (int i0 = begin + warp * 32; i0 < end; i0 += kWarps * 32) {
+      const int i = i0 + lane;
       int64_t page = -1;
-      int slot = 0;
+      int slot = 0, j = 0;
       if (i < end) {
         int64_t pi;
+        j = it.first + i * a.dilation;
         a.table.split(j, &pi, &slot);
         page = a.table.page_of(b, pi);
       }
@@ -293,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
       uint32_t seen[kRows];
 #pragma unroll
       for (int x = 0; x < kRows; ++x) {
-        const int64_t p = it.p0 + (x < rows ? x / it.heads : 0);
+        const int p = it.p0 + (x < rows ? x / it.heads : 0);
         const bool on = there && x < rows && (a.dilation > 1 || (j <= p && j > p - a.window));
         seen[x] = __ballot_sync(0xffffffffu, on);
         s[x] = on ? s[x] * k_scale * a.scale_log2 : -INFINITY;
@@ -313,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
         for (int e = 0; e < kD32; ++e) acc[x][e] *= keep;
         s[x] *= v_scale;
       }
-      const int count = (int)min((int64_t)32, end - i0);
+      const int count = min(32, end - i0);
       for (int key = 0; key < count; ++key) {
         const int64_t off = __shfl_sync(0xffffffffu, v_at, key);
         const bool has = __shfl_sync(0xffffffffu, (int)there, key);
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
-    leave<T>(a, it, part, o, a.D, ml, kRows);
+    leave<T, 1>(a, it, part, o, a.D, ml, kRows);
     at = stop;
   }
 }
@@ -417,20 +449,32 @@ template <int kDP, bool k8> struct Tile {
   static constexpr int kKeys = kRowBytes >= 256 ? 16 : 32;
   static constexpr int kStages = 3;
   static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
+  static constexpr int kStage = 2 * kMatrix;
   static constexpr int kExtra = 16 + (k8 ? 2 * kKeys * 4 : 0);     // which keys are there; scales
-  static constexpr int kStage = 2 * kMatrix + kExtra;
   static constexpr int kRows = 16;
   static size_t bytes(int D) {
-    const size_t tiles = (size_t)kWarps * kStages * kStage, merge = (size_t)kWarps * kRows * (D + 8) * sizeof(float);
+    const size_t tiles = (size_t)kWarps * kStages * (kStage + kExtra);
+    const size_t merge = (size_t)kWarps * kRows * (D + 8) * sizeof(float);
     return tiles > merge ? tiles : merge;
   }
-  // Chunks of a row are permuted so that eight neighbouring rows have any one chunk in eight different
-  // groups of banks.
+  // Byte of a chunk in a tile. Chunks of a row are permuted so that eight neighbouring rows have any one
+  // chunk in eight different groups of banks; at(row, c ^ x) == at(row, c) ^ (x << 4).
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
-    const int x = kChunks >= 8 ? row & 7 : kChunks == 4 ? row >> 1 & 3 : row >> 2 & 1;
+    const int x = kChunks >= 8 ? row & 7 : row >> 1 & 3;
     return row * kRowBytes + ((chunk ^ x) << 4);
   }
 };
+
+// The first n bits.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+}
+// Elements that are not finite (of a 32-bit word), as a mask over the word. 8 bits: e4m3 has a NaN only.
+template <class T, bool k8> __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  if (k8) return __vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  return __vcmpeq2(x & e, e);
+}
 
 template <class T, bool k8, int kDP>
 __global__ void __launch_bounds__(kThreads, kDP == 256 && !k8 ? 1 : 2)
@@ -438,85 +482,104 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   using M = typename std::conditional<k8, __half, T>::type;        // operands of the products
   using L = Tile<kDP, k8>;
   constexpr int kKeys = L::kKeys, kStages = L::kStages, kGroups = kKeys / 16, kSteps = kDP / 16;
-  extern __shared__ __align__(128) uint8_t tiles[];
+  constexpr int kElem = k8 ? 1 : 2;
+  extern __shared__ __align__(1024) uint8_t tiles[];
   __shared__ float2 ml[kWarps * 16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = lane >> 2, c = lane & 3;                          // rows r0, r0 + 8 and columns 2c, 2c + 1
-  uint8_t* const mine = tiles + warp * kStages * L::kStage;
-  const uint32_t mine_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
-  constexpr int kElem = k8 ? 1 : 2;
-  const int real_chunks = a.D * kElem / 16;
+  uint8_t* const my_tiles = tiles + warp * kStages * L::kStage;
+  uint8_t* const my_extra = tiles + kWarps * kStages * L::kStage + warp * kStages * L::kExtra;
+  const uint32_t tiles_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_tiles));
+  const uint32_t extra_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_extra));
+  // Copies: four lanes to a key, 64 bytes of its row at a time. Fragments: see the uses.
+  const uint32_t copy_off = L::at(r0, c);
+  const uint32_t key_off = k8 ? L::at(lane & 15, lane >> 4) : L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
+  const uint32_t value_off = L::kMatrix + L::at(lane & 15, lane >> 4);
+  const int my_chunks = a.D * kElem / 16 - c;                      // chunks c, c + 4, .. that a row has
 
   const Range r = my_range(a);
-  int b = r.b;
-  int64_t before = r.before;
-  for (int64_t at = r.begin; at < r.end;) {
-    const int length = a.lengths[b];
-    const int64_t units = units_of(a, length);
-    const int64_t index = (at - before) / units;
+  int b = r.b, length = r.length;
+  uint32_t before = r.before;
+  for (uint32_t at = r.begin; at < r.end;) {
+    const uint32_t units = units_of(a, length), index = (at - before) / units;
     if (index >= a.items) {
       before += units * a.items;
-      ++b;
+      length = a.lengths[++b];
       continue;
     }
     const Item it = item_of(a, b, index, length);
-    const int64_t item_begin = before + index * units, item_end = item_begin + units;
-    const int64_t stop = item_end < r.end ? item_end : r.end;
+    const uint32_t item_begin = before + index * units, item_end = item_begin + units;
+    const uint32_t stop = min(item_end, r.end);
     const int rows = it.tokens * it.heads;
-    const int64_t begin = (at - item_begin) * a.unit + warp * kKeys;
-    const int64_t end = min((stop - item_begin) * a.unit, it.n);
-    const int count = end > begin ? (int)((end - begin + a.unit - 1) / a.unit) : 0;   // of this warp's tiles
+    const int begin = (at - item_begin) * a.unit + warp * kKeys;
+    const int end = (int)min((int64_t)(stop - item_begin) * a.unit, (int64_t)it.n);
+    const int count = end > begin ? (end - begin + a.step - 1) / a.step : 0;          // this warp's tiles
+    const uint8_t* const k_base = static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem;
+    const uint8_t* const v_base = static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem;
+    const int* const table = a.table.entry + b * a.table.stride;
 
-    // the table's entry for this lane's key of tile `s`
-    const auto entry = [&](int s, int64_t* page, int* slot) {
-      const int64_t i = begin + (int64_t)s * a.unit + (lane & (kKeys - 1));
-      *page = -1;
-      *slot = 0;
+    // Page and slot of this lane's key of tile `s`; page -1: there is none. Looked up a tile before its
+    // copies are issued.
+    int page, slot;
+    const auto look_up = [&](int s) {
+      const int i = begin + s * a.step + (lane & (kKeys - 1));
+      page = -1;
+      slot = 0;
       if (s < count && i < end) {
-        int64_t pi;
-        a.table.split(it.first + i * a.dilation, &pi, slot);
-        *page = a.table.page_of(b, pi);
+        const uint32_t j = it.first + i * a.dilation;
+        uint32_t pi;
+        if (a.table.shift >= 0) {
+          pi = j >> a.table.shift;
+          slot = j & (a.table.page_size - 1);
+        } else {
+          pi = j / (uint32_t)a.table.page_size;
+          slot = j - pi * a.table.page_size;
+        }
+        if (pi < (uint32_t)a.table.max_pages) page = table[pi];
+        if ((uint32_t)page >= (uint32_t)a.table.pages) page = -1;
       }
     };
-    const auto fetch = [&](int s, int64_t page, int slot) {
-      const uint32_t base = mine_u32 + (s % kStages) * L::kStage;
-      const bool there = page >= 0;
-      int64_t k_at = -1, v_at = -1;
-      if (there) {
-        k_at = page * a.key.page + (int64_t)slot * a.key.token + it.head * a.key.head;
-        v_at = page * a.value.page + (int64_t)slot * a.value.token + it.head * a.value.head;
-      }
+    const auto fetch = [&](int s, int stage) {
       if (s < count) {
+        const bool there = page >= 0;
         const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(mine + (s % kStages) * L::kStage + 2 * L::kMatrix) = mask;
-        constexpr int kRowsAtOnce = 32 / L::kChunks;
-        const int chunk = lane % L::kChunks;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(my_extra + stage * L::kExtra) = mask;
+        int64_t k_at = -1, v_at = -1;
+        if (there) {
+          k_at = (page * a.key.page + slot * a.key.token) * kElem;
+          v_at = a.same_strides ? k_at : (page * a.value.page + slot * a.value.token) * kElem;
+        }
+        const uint32_t dst = tiles_at + stage * L::kStage + copy_off;
 #pragma unroll
-        for (int i = 0; i < kKeys / kRowsAtOnce; ++i) {
-          const int row = i * kRowsAtOnce + lane / L::kChunks;
-          const int64_t ka = __shfl_sync(0xffffffffu, k_at, row), va = __shfl_sync(0xffffffffu, v_at, row);
-          const bool ok = ka >= 0 && chunk < real_chunks;          // zeros elsewhere
-          const uint8_t* k = static_cast<const uint8_t*>(a.key.base) + (ok ? ka * kElem + chunk * 16 : 0);
-          const uint8_t* v = static_cast<const uint8_t*>(a.value.base) + (ok ? va * kElem + chunk * 16 : 0);
-          copy16(base + L::at(row, chunk), k, ok);
-          copy16(base + L::kMatrix + L::at(row, chunk), v, ok);
+        for (int g = 0; g < kKeys / 8; ++g) {
+          const int64_t ka = __shfl_sync(0xffffffffu, k_at, 8 * g + r0);
+          const int64_t va = a.same_strides ? ka : __shfl_sync(0xffffffffu, v_at, 8 * g + r0);
+          const uint8_t* const k = k_base + (ka >= 0 ? ka + c * 16 : 0);
+          const uint8_t* const v = v_base + (ka >= 0 ? va + c * 16 : 0);
+          const int chunks = ka >= 0 ? my_chunks : 0;              // zeros where there is nothing
+#pragma unroll
+          for (int i = 0; i < L::kChunks / 4; ++i) {
+            const bool ok = 4 * i < chunks;
+            const uint32_t to = (dst ^ (i << 6)) + 8 * g * L::kRowBytes;
+            copy16(to, ok ? k + i * 64 : k_base, ok);
+            copy16(to + L::kMatrix, ok ? v + i * 64 : v_base, ok);
+          }
         }
         if (k8 && lane < kKeys) {
-          const int64_t ks = there ? page * a.key.s_page + (int64_t)slot * a.key.s_token + it.head * a.key.s_head : 0;
-          const int64_t vs = there ? page * a.value.s_page + (int64_t)slot * a.value.s_token + it.head * a.value.s_head : 0;
-          copy4(base + 2 * L::kMatrix + 16 + lane * 4, a.key.scale + ks, there);
-          copy4(base + 2 * L::kMatrix + 16 + (kKeys + lane) * 4, a.value.scale + vs, there);
+          const int64_t ks = there ? page * a.key.s_page + slot * a.key.s_token + it.head * a.key.s_head : 0;
+          const int64_t vs = there ? page * a.value.s_page + slot * a.value.s_token + it.head * a.value.s_head : 0;
+          const uint32_t to = extra_at + stage * L::kExtra + 16 + lane * 4;
+          copy4(to, a.key.scale + ks, there);
+          copy4(to + kKeys * 4, a.value.scale + vs, there);
         }
       }
       copy_commit();
     };
-    int64_t page;
-    int slot;
-    entry(0, &page, &slot);
+    look_up(0);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
-      fetch(s, page, slot);
-      entry(s + 1, &page, &slot);
+      fetch(s, s);
+      look_up(s + 1);
     }
 
     // The queries as A fragments: rows r0 and r0 + 8. 16-bit caches: channels 16 k + 2c, + 1 and 8 further;
@@ -533,37 +596,51 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         const int t = it.t0 + row_token[x], h = it.head * a.group + it.h0 + row % it.heads;
         src = static_cast<const T*>(a.query) + b * a.q_batch + t * a.q_token + h * a.q_head;
       }
-      T v[kSteps][4];
+      Elements<T, 2> v[kSteps][2];
 #pragma unroll
       for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 16 * k + (k8 ? 4 * c + e : 2 * c + (e & 1) + 8 * (e >> 1));
-          v[k][e] = src && d < a.D ? src[d] : from_float<T>(0.f);
+        for (int e = 0; e < 2; ++e) {
+          const int d = 16 * k + (k8 ? 4 * c + 2 * e : 2 * c + 8 * e);
+          if (!src || d >= a.D) v[k][e].v[0] = v[k][e].v[1] = from_float<T>(0.f);
+          else if (a.q_words) v[k][e] = *reinterpret_cast<const Elements<T, 2>*>(src + d);
+          else {
+            v[k][e].v[0] = src[d];
+            v[k][e].v[1] = src[d + 1];
+          }
         }
-      float factor = 1.f;
       row_scale[x] = a.scale_log2;
-      if (k8) {
+      if constexpr (k8) {
         float most = 0.f;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(as_float(v[k][e])));
+          for (int e = 0; e < 2; ++e)
+            most = fmaxf(most, fmaxf(fabsf(as_float(v[k][e].v[0])), fabsf(as_float(v[k][e].v[1]))));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         // 2^-e and 2^e of the largest magnitude's exponent, where both are normal numbers
         const int e = (__float_as_int(most) >> 23) - 127;
+        float factor = 1.f;
         if (e > -126 && e < 127) {
           factor = __int_as_float((127 - e) << 23);
           row_scale[x] *= __int_as_float((127 + e) << 23);
         }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2)
+            q[k][x + 2 * e2] = Half2Of<M>::pack(as_float(v[k][e2].v[0]) * factor, as_float(v[k][e2].v[1]) * factor);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) q[k][x + 2 * e] = *reinterpret_cast<const uint32_t*>(&v[k][e]);
       }
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          q[k][x + 2 * e] = Half2Of<M>::pack(as_float(v[k][2 * e]) * factor, as_float(v[k][2 * e + 1]) * factor);
     }
+    // Tiles whose first key lies in [safe_from, safe_to] are attended whole, or not, by all rows alike.
+    const bool alike = it.tokens == 1;
+    const int64_t safe_from = (int64_t)it.p0 + it.tokens - a.window, safe_to = (int64_t)it.p0 - kKeys + 1;
 
     float acc[kDP / 8][4], m[2], l[2], mv[2];
 #pragma unroll
@@ -576,30 +653,38 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       l[x] = 0.f;
     }
 
+    int stage = 0;
+#pragma unroll 1
     for (int s = 0; s < count; ++s) {
       copy_wait<kStages - 2>();
       __syncwarp();                        // the tile is there, and everyone is done with the one before it
-      fetch(s + kStages - 1, page, slot);
-      entry(s + kStages, &page, &slot);
-      const uint32_t base = mine_u32 + (s % kStages) * L::kStage;
-      const uint8_t* extra = mine + (s % kStages) * L::kStage + 2 * L::kMatrix;
-      uint32_t there = *reinterpret_cast<const uint32_t*>(extra);
-      if (kKeys < 32) there &= (1u << (kKeys & 31)) - 1;
+      fetch(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+      look_up(s + kStages);
+      const uint32_t base = tiles_at + stage * L::kStage;
+      const uint8_t* extra = my_extra + stage * L::kExtra;
+      uint8_t* const values = my_tiles + stage * L::kStage + L::kMatrix;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
 
-      float p[2 * kGroups][4];
+      // p = queries x keys: columns 8 i + 2c, + 1 of rows r0 (0, 1) and r0 + 8 (2, 3). With 16 keys the sums
+      // over the channels go in two, so that no chain of products is longer than four.
+      constexpr int kChains = kGroups == 1 ? 2 : 1;
+      float part[kChains][2 * kGroups][4];
 #pragma unroll
-      for (int i = 0; i < 2 * kGroups; ++i)
+      for (int z = 0; z < kChains; ++z)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[i][e] = 0.f;
+        for (int i = 0; i < 2 * kGroups; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[z][i][e] = 0.f;
+      const uint32_t keys = base + key_off;
       if constexpr (!k8) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) {
             uint32_t f[4];
-            ldmatrix4<false>(f, base + L::at(16 * g + (lane & 7) + (lane >> 4) * 8, 2 * k + (lane >> 3 & 1)));
-            mma<M>(p[2 * g], q[k], f[0], f[1]);
-            mma<M>(p[2 * g + 1], q[k], f[2], f[3]);
+            ldmatrix4<false>(f, (keys ^ (k << 5)) + 16 * g * L::kRowBytes);
+            mma<M>(part[k % kChains][2 * g], q[k], f[0], f[1]);
+            mma<M>(part[k % kChains][2 * g + 1], q[k], f[2], f[3]);
           }
       } else {
 #pragma unroll
@@ -607,63 +692,68 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) {
             uint32_t f[4];
-            ldmatrix4<false>(f, base + L::at(16 * g + (lane & 15), k + (lane >> 4)));
+            ldmatrix4<false>(f, (keys ^ (k << 4)) + 16 * g * L::kRowBytes);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-              mma<M>(p[2 * g], q[k + z], e4m3_to_f16(f[2 * z]), e4m3_to_f16(f[2 * z] >> 16));
-              mma<M>(p[2 * g + 1], q[k + z], e4m3_to_f16(f[2 * z + 1]), e4m3_to_f16(f[2 * z + 1] >> 16));
+              mma<M>(part[z % kChains][2 * g], q[k + z], e4m3_to_f16(f[2 * z]), e4m3_to_f16(f[2 * z] >> 16));
+              mma<M>(part[z % kChains][2 * g + 1], q[k + z], e4m3_to_f16(f[2 * z + 1]), e4m3_to_f16(f[2 * z + 1] >> 16));
             }
           }
       }
-
-      // which keys each row attends
-      const int64_t i0 = begin + (int64_t)s * a.unit;
-      const int64_t j0 = it.first + i0 * a.dilation;
-      const bool differ = it.tokens > 1 && !(j0 + kKeys - 1 <= it.p0 && j0 > it.p0 + it.tokens - 1 - a.window);
-      constexpr uint32_t kAll = kKeys < 32 ? (1u << (kKeys & 31)) - 1 : 0xffffffffu;
-      uint32_t on[2] = {there, there};
-      if (differ) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          // keys j <= p: the first p - j0 + 1; keys j > p - window: not the first p - window - j0 + 1
-          const int64_t pos = it.p0 + row_token[x] - j0;
-          const int64_t upto = pos + 1, from = pos - a.window + 1;
-          on[x] &= upto <= 0 ? 0u : upto >= 32 ? 0xffffffffu : (1u << (int)upto) - 1;
-          on[x] &= from <= 0 ? 0xffffffffu : from >= 32 ? 0u : ~((1u << (int)from) - 1);
-        }
-      }
-      const float* k_scale = reinterpret_cast<const float*>(extra + 16);
-      const float* v_scale = k_scale + kKeys;
-      float top[2] = {-INFINITY, -INFINITY}, lv[2 * kGroups][2];
+      float p[2 * kGroups][4], lv[2 * kGroups][2];
 #pragma unroll
       for (int i = 0; i < 2 * kGroups; ++i) {
-        float2 ks = make_float2(1.f, 1.f);
-        if (k8) {
-          ks = *reinterpret_cast<const float2*>(k_scale + 8 * i + 2 * c);
-          const float2 vs = *reinterpret_cast<const float2*>(v_scale + 8 * i + 2 * c);
-          lv[i][0] = __log2f(vs.x);
-          lv[i][1] = __log2f(vs.y);
-        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[i][e] *= k8 ? row_scale[e >> 1] * (e & 1 ? ks.y : ks.x) : row_scale[e >> 1];
-          if (on[e >> 1] != kAll && !(on[e >> 1] >> (8 * i + 2 * c + (e & 1)) & 1)) p[i][e] = -INFINITY;
-          top[e >> 1] = fmaxf(top[e >> 1], p[i][e]);
+          p[i][e] = part[0][i][e];
+          if (kChains == 2) p[i][e] += part[kChains - 1][i][e];
+        }
+        if constexpr (k8) {
+          const float2 ks = *reinterpret_cast<const float2*>(extra + 16 + (8 * i + 2 * c) * 4);
+          const float2 vs = *reinterpret_cast<const float2*>(extra + 16 + (kKeys + 8 * i + 2 * c) * 4);
+          lv[i][0] = __log2f(vs.x);
+          lv[i][1] = __log2f(vs.y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[i][e] *= e & 1 ? ks.y : ks.x;
         }
       }
-      float topv[2] = {-INFINITY, -INFINITY};
-      if (k8) {
+
+      // which keys each row attends
+      const uint32_t there = *reinterpret_cast<const uint32_t*>(extra) & first_bits(kKeys);
+      const int j0 = it.first + (begin + s * a.step) * a.dilation;
+      const bool differ = !alike && !(j0 >= safe_from && j0 <= safe_to);
+      if (there != first_bits(kKeys) || differ) {
+        uint32_t on[2] = {there, there};
+        if (differ) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int upto = it.p0 + row_token[x] - j0 + 1;        // keys j <= p and j > p - window
+            const int64_t from = upto - a.window;
+            on[x] &= first_bits(upto) & ~first_bits(from > 0 ? (int)min(from, (int64_t)32) : 0);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 2 * kGroups; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) topv[e >> 1] = fmaxf(topv[e >> 1], p[i][e] + lv[i][e & 1]);
+          for (int e = 0; e < 4; ++e)
+            if (!(on[e >> 1] >> (8 * i + 2 * c + (e & 1)) & 1)) p[i][e] = -INFINITY;
       }
+
+      // the running maximum of the logits (and of the logits with the values' scales)
       float base_m[2], base_v[2], keep[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        const float next = fmaxf(m[x], top[x]);
+        float top = -INFINITY, topv = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2 * kGroups; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            top = fmaxf(top, p[i][2 * x + e]);
+            if (k8) topv = fmaxf(topv, fmaf(p[i][2 * x + e], row_scale[x], lv[i][e]));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float next = fmaxf(m[x], top * row_scale[x]);
         // nothing attended yet: no difference of infinities. (A NaN logit is passed over by the maximum and
         // comes back in the exponential.)
         base_m[x] = next == -INFINITY ? 0.f : next;
@@ -671,15 +761,15 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         l[x] *= keep[x];
         m[x] = next;
         if (k8) {
-          topv[x] = fmaxf(topv[x], __shfl_xor_sync(0xffffffffu, topv[x], 1));
-          topv[x] = fmaxf(topv[x], __shfl_xor_sync(0xffffffffu, topv[x], 2));
-          const float nextv = fmaxf(mv[x], topv[x]);
+          topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
+          topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
+          const float nextv = fmaxf(mv[x], topv);
           base_v[x] = nextv == -INFINITY ? 0.f : nextv;
           keep[x] = ex2(mv[x] - base_v[x]);
           mv[x] = nextv;
         }
       }
-      if (keep[0] != 1.f || keep[1] != 1.f) {
+      if (__any_sync(0xffffffffu, !(keep[0] == 1.f && keep[1] == 1.f))) {
 #pragma unroll
         for (int i = 0; i < kDP / 8; ++i)
 #pragma unroll
@@ -691,62 +781,75 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = p[i][e];
-          const float ex = ex2(x - base_m[e >> 1]);
-          l[e >> 1] += ex;
-          y[e] = k8 ? ex2(x + lv[i][e & 1] - base_v[e >> 1]) : ex;
-          // a token left out has the scale 0 or any other: its weight is 0
-          if (k8 && x == -INFINITY) y[e] = 0.f;
+          const int x = e >> 1;
+          const float ex = ex2(fmaf(p[i][e], row_scale[x], -base_m[x]));
+          l[x] += ex;
+          y[e] = k8 ? ex2(fmaf(p[i][e], row_scale[x], lv[i][e & 1]) - base_v[x]) : ex;
+          if (k8 && p[i][e] == -INFINITY) y[e] = 0.f;              // left out, whatever its scale is
         }
         w[i >> 1][2 * (i & 1)] = Half2Of<M>::pack(y[0], y[1]);
         w[i >> 1][2 * (i & 1) + 1] = Half2Of<M>::pack(y[2], y[3]);
       }
 
+      // Rows attend different keys of this tile: 0 x NaN of a value must not reach the rows that do not
+      // attend it. Values that are not finite (hardly ever any) go straight to the sums of the rows that
+      // do, whatever their weights, and become zeros in the tile.
+      if (differ) {
+        uint32_t bad = 0;
+        for (int i = lane; i < L::kMatrix / 4; i += 32)
+          if (not_finite<T, k8>(reinterpret_cast<const uint32_t*>(values)[i])) bad |= 1u << (i / (L::kRowBytes / 4));
+        bad = __reduce_or_sync(0xffffffffu, bad) & there;
+        for (; bad; bad &= bad - 1) {
+          const int key = __ffs(bad) - 1, upto = it.p0 - j0 - key;          // p0 - j
+#pragma unroll
+          for (int i = 0; i < L::kChunks; ++i) {
+            uint32_t* const at_word = reinterpret_cast<uint32_t*>(values + L::at(key, i) + 4 * c);
+            const uint32_t word = *at_word, odd = not_finite<T, k8>(word);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int back = upto + row_token[x];                         // p - j
+              if (back < 0 || back >= a.window) continue;
+#pragma unroll
+              for (int e = 0; e < 4 / kElem; ++e) {
+                if (!(odd >> (8 * kElem * e) & 1)) continue;
+                float y = __int_as_float(0x7fc00000);
+                if (!k8) {
+                  const uint16_t bits = word >> (16 * e);
+                  y = as_float(*reinterpret_cast<const T*>(&bits));
+                }
+                acc[k8 ? 2 * i + (e & 1) : i][2 * x + (k8 ? e >> 1 : e)] += y;
+              }
+            }
+            __syncwarp();
+            if (odd && r0 == 0) *at_word = word & ~odd;
+          }
+        }
+        __syncwarp();
+      }
+
       // values: B fragments of two (8-bit: four) 8-channel columns for 16 keys at a time
+      const uint32_t vals = base + value_off;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const auto column = [&](int n, uint32_t b0, uint32_t b1) {
-          if (!differ) {
-            mma<M>(acc[n], w[g], b0, b1);
-          } else {
-            // Rows attend different keys of this tile: a NaN or an infinity of a value must stay with the
-            // rows that attend it, so every query token gets the values with the others' taken out.
-            for (int t = 0; t < it.tokens; ++t) {
-              const int64_t pos = it.p0 + t - j0;
-              const int64_t upto = pos + 1, from = pos - a.window + 1;
-              uint32_t seen = there;
-              seen &= upto <= 0 ? 0u : upto >= 32 ? 0xffffffffu : (1u << (int)upto) - 1;
-              seen &= from <= 0 ? 0xffffffffu : from >= 32 ? 0u : ~((1u << (int)from) - 1);
-              seen >>= 16 * g + 2 * c;
-              const uint32_t s0 = (seen & 1 ? 0xffffu : 0u) | (seen & 2 ? 0xffff0000u : 0u);
-              const uint32_t s1 = (seen >> 8 & 1 ? 0xffffu : 0u) | (seen >> 8 & 2 ? 0xffff0000u : 0u);
-              float part[4] = {0.f, 0.f, 0.f, 0.f};
-              mma<M>(part, w[g], b0 & s0, b1 & s1);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (row_token[e >> 1] == t) acc[n][e] += part[e];
-            }
-          }
-        };
         if constexpr (!k8) {
 #pragma unroll
           for (int n = 0; n < kSteps; ++n) {
             uint32_t f[4];
-            ldmatrix4<true>(f, base + L::kMatrix + L::at(16 * g + (lane & 15), 2 * n + (lane >> 4)));
-            column(2 * n, f[0], f[1]);
-            column(2 * n + 1, f[2], f[3]);
+            ldmatrix4<true>(f, (vals ^ (n << 5)) + 16 * g * L::kRowBytes);
+            mma<M>(acc[2 * n], w[g], f[0], f[1]);
+            mma<M>(acc[2 * n + 1], w[g], f[2], f[3]);
           }
         } else {
           // a 16-bit unit holds channels d, d + 1 of a key: sorted into pairs of keys for d and for d + 1
 #pragma unroll
           for (int n = 0; n < kSteps; n += 2) {
             uint32_t f[4];
-            ldmatrix4<true>(f, base + L::kMatrix + L::at(16 * g + (lane & 15), n + (lane >> 4)));
+            ldmatrix4<true>(f, (vals ^ (n << 4)) + 16 * g * L::kRowBytes);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const uint32_t lo = f[2 * z], hi = f[2 * z + 1];
-              column(2 * (n + z), e4m3_to_f16(__byte_perm(lo, 0, 0x4420)), e4m3_to_f16(__byte_perm(hi, 0, 0x4420)));
-              column(2 * (n + z) + 1, e4m3_to_f16(__byte_perm(lo, 0, 0x4431)), e4m3_to_f16(__byte_perm(hi, 0, 0x4431)));
+              mma<M>(acc[2 * (n + z)], w[g], e4m3_to_f16(__byte_perm(lo, 0, 0x4420)), e4m3_to_f16(__byte_perm(hi, 0, 0x4420)));
+              mma<M>(acc[2 * (n + z) + 1], w[g], e4m3_to_f16(__byte_perm(lo, 0, 0x4431)), e4m3_to_f16(__byte_perm(hi, 0, 0x4431)));
             }
           }
         }
@@ -785,46 +888,60 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
-    leave<T>(a, it, part, o, o_stride, ml, 16);
+    leave<T, 4>(a, it, part, o, o_stride, ml, 16);
     __syncthreads();                                               // before the next item's tiles come
     at = stop;
   }
 }
 
 // ---- the join --------------------------------------------------------------------------------------------
-// A warp per row of an item; items that one block had are done.
+// A warp per row of an item; items that one block had are done. A lane has a part's maximum and sum, then the
+// lanes share the channels.
 template <class T>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a,
                                                                int rows_max) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int64_t id = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) / rows_max;
-  const int row = (int)(((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) - id * rows_max);
-  if (id >= a.B * a.items) return;
+  const uint32_t id_row = blockIdx.x * kWarps + (threadIdx.x >> 5), id = id_row / rows_max;
+  const int row = (int)(id_row - id * rows_max);
+  const bool mine = id < a.B * a.items;
+  const int b = id / a.items;
+  const Item it = rows_of(a, b, id - b * a.items);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine || row >= it.tokens * it.heads) return;
   const int2 covered = a.covered[id];
   if (covered.y <= 1) return;
-  const int b = (int)(id / a.items);
-  const Item it = item_of(a, b, id - b * a.items, a.lengths[b]);
-  if (row >= it.tokens * it.heads) return;
   // the first block's part is its second one (the item began there), the others' their first
   const auto slot = [&](int i) {
     return (int64_t)(2 * (covered.x + i) + (i == 0 ? 1 : 0)) * rows_max + row;
   };
-  float m = -INFINITY;
-  for (int i = lane; i < covered.y; i += 32) m = fmaxf(m, a.part_ml[slot(i)].x);
-  for (int f = 16; f > 0; f >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, f));
-  float l = 0.f, acc[8];
+  float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  for (int i = 0; i < covered.y; ++i) {
-    const float2 p = a.part_ml[slot(i)];
-    if (p.x == -INFINITY) continue;
-    const float f = exp2f(p.x - m);
-    l += f * p.y;
-    const float* o = a.part_o + slot(i) * a.D;
+  for (int i0 = 0; i0 < covered.y; i0 += 32) {
+    const int count = min(32, covered.y - i0);
+    const float2 p = lane < count ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    float top = p.x;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < a.D) acc[e] += f * o[lane + 32 * e];
+    for (int f = 16; f > 0; f >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, f));
+    const float next = fmaxf(m, top), base = next == -INFINITY ? 0.f : next;
+    const float keep = exp2f(m - base);
+    const float w = p.x == -INFINITY ? 0.f : exp2f(p.x - base);
+    float sum = p.x == -INFINITY ? 0.f : w * p.y;
+#pragma unroll
+    for (int f = 16; f > 0; f >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, f);
+    l = l * keep + sum;
+    m = next;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const float f = __shfl_sync(0xffffffffu, w, i), top_i = __shfl_sync(0xffffffffu, p.x, i);
+      const float* o = a.part_o + slot(i0 + i) * a.D;
+      if (top_i == -INFINITY) continue;         // nothing was written
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (lane + 32 * e < a.D) acc[e] += f * o[lane + 32 * e];
+    }
   }
   const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
   const int64_t at = ((int64_t)b * a.T + t) * a.Hq + h;
@@ -840,7 +957,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
 struct Plan {
   bool tensor_cores;
   int rows_max;             // rows of an item
-  int unit;
+  int step, unit;
   int item_tokens, item_heads, token_blocks, head_blocks, parts;
   int64_t items;
   int64_t covered_bytes, ml_bytes, o_bytes;
@@ -869,19 +986,22 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   p->tensor_cores = reads_in_chunks(*cache, dtype);
   p->rows_max = p->tensor_cores ? 16 : group == 1 && (T <= 1 || dilation > 1) ? 1 : 8;
   // a tile for each of a block's warps
-  p->unit = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
+  p->step = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
   p->item_heads = group < p->rows_max ? group : p->rows_max;
   p->head_blocks = (group + p->item_heads - 1) / p->item_heads;
   p->item_tokens = dilation > 1 ? 1 : p->rows_max / p->item_heads;
   if (p->item_tokens > T) p->item_tokens = T < 1 ? 1 : T;
   p->token_blocks = (T + p->item_tokens - 1) / p->item_tokens;
   p->items = (int64_t)cache->heads * p->token_blocks * p->head_blocks;
-  if (B > 0 && p->items > ((int64_t)1 << 31) / B) return B200NA_ERR_INVALID_ARGUMENT;
-  // units if every sequence were as long as the table allows
+  if (B > 0 && p->items * p->rows_max > (int64_t)0x7fffffff / B) return B200NA_ERR_INVALID_ARGUMENT;
+  // units if every sequence were as long as the table allows: larger ones where 31 bits would not count them
   int64_t most = (int64_t)max_pages * cache->page_size;
+  if (most > 0x7fffffff - 4096) return B200NA_ERR_UNSUPPORTED;
   if (kernel > 0 && most > (int64_t)kernel + p->item_tokens) most = (int64_t)kernel + p->item_tokens;
+  p->unit = p->step;
+  while (B * p->items * (most / p->unit + 1) > 0x7fffffff && p->unit <= most) p->unit *= 2;
   const int64_t units = B * p->items * (most / p->unit + 1);
-  if (most / p->unit + 1 > ((int64_t)1 << 52) / (B * p->items + 1)) return B200NA_ERR_INVALID_ARGUMENT;
+  if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   p->parts = (int)(units < kMostParts ? (units < 1 ? 1 : units) : kMostParts);
   p->covered_bytes = round_up(B * p->items * (int64_t)sizeof(int2));
   p->ml_bytes = round_up((int64_t)2 * p->parts * p->rows_max * sizeof(float2));
@@ -950,9 +1070,8 @@ int run(const DecodeArgs& a, bool tensor_cores, int cache_dtype, int rows_max, c
   // The join's blocks may take their places while the first launch's last ones run (they wait for its end
   // before they read anything).
   cudaLaunchConfig_t cfg{};
-  const int64_t warps = a.B * a.items * rows_max;
+  const int64_t warps = (int64_t)a.B * a.items * rows_max;
   const int64_t blocks = (warps + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
@@ -989,7 +1108,7 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   if (!query_strides || !(scale > 0.f) || !(scale < INFINITY)) return B200NA_ERR_INVALID_ARGUMENT;
   if (B == 0 || T == 0) return B200NA_OK;
   if (!query || !out || !lengths || !workspace) return B200NA_ERR_INVALID_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200NA_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) % 16) return B200NA_ERR_ALIGNMENT;
   DecodeArgs a{};
   a.query = query;
   a.q_batch = B > 1 ? query_strides[0] : 0;
@@ -1001,7 +1120,7 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.value = paged_pool(*cache, true);
   a.table = page_table(*cache, table, table_stride, max_pages);
   a.lengths = lengths;
-  a.capacity = (int64_t)max_pages * cache->page_size;
+  a.capacity = cache->pages > 0 ? max_pages * cache->page_size : 0;
   a.B = B;
   a.T = T;
   a.Hq = Hq;
@@ -1015,9 +1134,12 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.item_heads = p.item_heads;
   a.token_blocks = p.token_blocks;
   a.head_blocks = p.head_blocks;
-  a.items = p.items;
+  a.items = (uint32_t)p.items;
   a.parts = p.parts;
+  a.step = p.step;
   a.unit = p.unit;
+  a.q_words = reinterpret_cast<uintptr_t>(query) % 4 == 0 && (a.q_batch | a.q_token | a.q_head) % 2 == 0;
+  a.same_strides = a.key.page == a.value.page && a.key.token == a.value.token;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.covered = reinterpret_cast<int2*>(w);
   a.part_ml = reinterpret_cast<float2*>(w + p.covered_bytes);
