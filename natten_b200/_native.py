@@ -26,3 +26,5 @@ def _load():
 
 _module = _load()
 na, attention, layer, tiles = _module.na, _module.attention, _module.layer, _module.tiles
+rotary, na1d_decode = _module.rotary, _module.na1d_decode
+kv_cache_write, kv_cache_read = _module.kv_cache_write, _module.kv_cache_read

@@ -18,9 +18,11 @@
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -51,7 +53,8 @@ constexpr int kMaxDim = 3;
 #define B200NA_FUNCTIONS(X)                                                                  \
   X(na_forward_view) X(na_forward_simt) X(fmha_forward) X(fmha_splits) X(fmha_forward_split)  \
   X(na_backward_view) X(na_backward_simt)                                                     \
-  X(column_sum) X(column_sum_scratch) X(strerror)
+  X(column_sum) X(column_sum_scratch) X(strerror)                                             \
+  X(rotary) X(kv_cache_write) X(kv_cache_read) X(na1d_decode) X(na1d_decode_workspace)
 struct Lib {
 #define X(name) decltype(&b200na_##name) name = nullptr;
   B200NA_FUNCTIONS(X)
@@ -1176,6 +1179,372 @@ PyObject* py_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions -------------------------------------------------------------------------------
+
+struct RotaryCall : torch::CustomClassHolder {
+  int nd = 0, axes = 0;
+  std::array<int, kMaxDim> dims{0, 0, 0};
+  std::array<double, kMaxDim> theta{1, 1, 1}, scale{1, 1, 1};
+  std::array<int64_t, kMaxDim> origin{0, 0, 0};
+  int position_type = 0;
+  bool interleaved = false, has_key = false, has_positions = false;
+};
+
+// {query, key} (key only where there is one) turned; `inverse` turns back. Any strides.
+variable_list rotary_now(const RotaryCall& c, Tensor q, Tensor k, const Tensor& positions_, bool inverse) {
+  c10::cuda::CUDAGuard guard(q.device());
+  const auto readable = [](const Tensor& t) {
+    return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+  };
+  q = readable(q);
+  k = readable(k);
+  const Tensor at = positions_.defined() ? positions_.contiguous() : positions_;
+  variable_list out{at::empty(q.sizes(), q.options())};
+  if (k.defined()) out.push_back(at::empty(k.sizes(), k.options()));
+  if (q.numel() == 0) return out;
+  std::array<int, kMaxDim> shape{1, 1, 1};
+  for (int i = 0; i < c.nd; ++i) shape[i] = (int)q.size(1 + i);
+  check(lib.rotary(q.data_ptr(), k.defined() ? k.data_ptr() : nullptr, out[0].data_ptr(),
+                   k.defined() ? out[1].data_ptr() : nullptr, c.nd, shape.data(), (int)q.size(0),
+                   (int)q.size(-2), k.defined() ? (int)k.size(-2) : 0, (int)q.size(-1),
+                   dtype_code(q.scalar_type()), q.strides().data(),
+                   k.defined() ? k.strides().data() : nullptr, c.axes, c.dims.data(), c.theta.data(),
+                   c.scale.data(), c.origin.data(), at.defined() ? at.data_ptr() : nullptr, c.position_type,
+                   at.defined() && at.size(0) > 1, c.interleaved, inverse, stream_of(q)),
+        "b200na_rotary");
+  ++launches;
+  return out;
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  // in: the query, the key where there is one, the positions where there are any
+  static variable_list forward(AutogradContext* ctx, at::TensorList in,
+                               const c10::intrusive_ptr<RotaryCall>& call, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor positions = call->has_positions ? in[in.size() - 1] : Tensor();
+    if (call->has_positions) ctx->save_for_backward({positions});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
+    ctx->saved_data["inverse"] = inverse;
+    ctx->set_materialize_grads(false);
+    return rotary_now(*call, in[0], call->has_key ? in[1] : Tensor(), positions, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto call = c10::static_intrusive_pointer_cast<RotaryCall>(ctx->saved_data["call"].toCapsule());
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    const Tensor positions = call->has_positions ? ctx->get_saved_variables()[0] : Tensor();
+    variable_list g(1 + call->has_key + call->has_positions + 2);
+    // the outputs that have a gradient whose input wants one, turned back in one launch
+    std::vector<size_t> which;
+    for (size_t i = 0; i < (size_t)(1 + call->has_key); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) which.push_back(i);
+    if (which.empty()) return g;
+    const Tensor a = grads[which[0]], b = which.size() > 1 ? grads[which[1]] : Tensor();
+    variable_list turned;
+    if (c10::GradMode::is_enabled()) {     // to be differentiated again
+      auto again = c10::make_intrusive<RotaryCall>(*call);
+      again->has_key = b.defined();
+      variable_list in{a};
+      if (b.defined()) in.push_back(b);
+      if (positions.defined()) in.push_back(positions);
+      turned = RotaryFunction::apply(at::TensorList(in), again, inverse);
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      turned = rotary_now(*call, a, b, positions, inverse);
+    }
+    for (size_t i = 0; i < which.size(); ++i) g[which[i]] = turned[i];
+    return g;
+  }
+};
+
+bool parse_number(PyObject* o, double* out) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  *out = PyFloat_AsDouble(o);
+  if (*out == -1. && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return std::isfinite(*out);
+}
+bool parse_number(PyObject* o, int64_t* out) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  *out = PyLong_AsLongLongAndOverflow(o, &overflow);
+  return !overflow && *out > -(1ll << 53) && *out < (1ll << 53);
+}
+// one number for all axes, or one for each
+template <class N> bool parse_per_axis(PyObject* o, int axes, std::array<N, kMaxDim>* out) {
+  if (PyTuple_Check(o) || PyList_Check(o)) {
+    if (PySequence_Fast_GET_SIZE(o) != axes) return false;
+    for (int a = 0; a < axes; ++a)
+      if (!parse_number(PySequence_Fast_GET_ITEM(o, a), &(*out)[a])) return false;
+    return true;
+  }
+  if (!parse_number(o, &(*out)[0])) return false;
+  for (int a = 1; a < axes; ++a) (*out)[a] = (*out)[0];
+  return true;
+}
+bool rotary_type(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+
+// rotary(query, key, axis_dims, theta, positions, origin, position_scale, interleaved)
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "rotary() takes 8 arguments");
+  Tensor q, k, at;
+  if (!plain_mode() || !plain_tensor(a[0], &q) || (a[1] != Py_None && !plain_tensor(a[1], &k)) ||
+      (a[4] != Py_None && !plain_tensor(a[4], &at)) || !PyBool_Check(a[7]))
+    Py_RETURN_NONE;
+  if (q.dim() < 4 || q.dim() > 6 || !rotary_type(q) || q.size(-1) > 256 || q.size(-1) < 1 || q.size(-2) < 1 ||
+      q.size(-2) > 65536)
+    Py_RETURN_NONE;
+  for (int64_t s : q.sizes())
+    if (s > 0x7fffffff) Py_RETURN_NONE;
+  if (k.defined()) {
+    if (k.dim() != q.dim() || k.scalar_type() != q.scalar_type() || k.device() != q.device() ||
+        k.sizes().slice(0, k.dim() - 2) != q.sizes().slice(0, q.dim() - 2) || k.size(-1) != q.size(-1) ||
+        k.size(-2) < 1 || k.size(-2) > 65536)
+      Py_RETURN_NONE;
+  }
+  auto call = c10::make_intrusive<RotaryCall>();
+  RotaryCall& c = *call;
+  c.nd = c.axes = (int)q.dim() - 3;
+  c.interleaved = a[7] == Py_True;
+  c.has_key = k.defined();
+  c.has_positions = at.defined();
+  if (at.defined()) {
+    const auto t = at.scalar_type();
+    if ((t != at::kInt && t != at::kLong && t != at::kFloat) || at.dim() != q.dim() - 1 || at.size(-1) < 1 ||
+        at.size(-1) > 3 || at.device() != q.device() || (at.size(0) != 1 && at.size(0) != q.size(0)) ||
+        at.sizes().slice(1, c.nd) != q.sizes().slice(1, c.nd) || any_requires_grad({&at}))
+      Py_RETURN_NONE;
+    c.axes = (int)at.size(-1);
+    c.position_type = t == at::kInt ? 0 : t == at::kLong ? 1 : 2;
+  }
+  const int D = (int)q.size(-1);
+  if (a[2] == Py_None) {     // equal parts in steps of 8 channels, or of 2 (positions.py: rotary_axis_dims)
+    const int step = D % 8 == 0 && D >= 8 * c.axes ? 8 : 2, parts = D / step;
+    for (int i = 0; i < c.axes; ++i) c.dims[i] = step * (parts / c.axes + (i < parts % c.axes));
+  } else {
+    if (!(PyTuple_Check(a[2]) || PyList_Check(a[2])) || !parse_dims(a[2], c.axes, 0, 0, &c.dims)) Py_RETURN_NONE;
+    long long sum = 0;
+    for (int i = 0; i < c.axes; ++i) {
+      if (c.dims[i] % 2) Py_RETURN_NONE;
+      sum += c.dims[i];
+    }
+    if (sum > D) Py_RETURN_NONE;
+  }
+  if (!parse_per_axis(a[3], c.axes, &c.theta) || !parse_per_axis(a[5], c.axes, &c.origin) ||
+      !parse_per_axis(a[6], c.axes, &c.scale))
+    Py_RETURN_NONE;
+  for (int i = 0; i < c.axes; ++i)
+    if (!(c.theta[i] > 0.) || (at.defined() && c.origin[i] != 0)) Py_RETURN_NONE;
+  variable_list out;
+  if (any_requires_grad({&q, &k})) {
+    pybind11::gil_scoped_release no_gil;
+    variable_list in{q};
+    if (k.defined()) in.push_back(k);
+    if (at.defined()) in.push_back(at);
+    out = RotaryFunction::apply(at::TensorList(in), call, false);
+  } else {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = rotary_now(c, q, k, at, false);
+  }
+  return wrap(out[0], k.defined() ? out[1] : Tensor(), k.defined());
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- paged key/value cache -----------------------------------------------------------------------------
+
+struct Cache {
+  Tensor key, value, key_scale, value_scale;
+  b200na_kv_cache c{};
+};
+// A KVCache (kv_cache.py): a tuple of the pools and, in 8 bits, their scales.
+bool parse_cache(PyObject* o, Cache* out) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  Tensor* const t[4] = {&out->key, &out->value, &out->key_scale, &out->value_scale};
+  for (int i = 0; i < 4; ++i) {
+    PyObject* x = PyTuple_GET_ITEM(o, i);
+    if (i >= 2 && x == Py_None) continue;
+    if (!plain_tensor(x, t[i])) return false;
+  }
+  const Tensor &k = out->key, &v = out->value;
+  const int dt = dtype_code(k.scalar_type());
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() ||
+      k.device() != v.device() || dt < 0 || dt == B200NA_E5M2)
+    return false;
+  for (int i = 0; i < 4; ++i)
+    if (k.size(i) < (i ? 1 : 0) || k.size(i) > 0x7fffffff) return false;
+  if (k.size(3) > 256 || (k.size(3) > 1 && (k.stride(3) != 1 || v.stride(3) != 1))) return false;
+  if (out->key_scale.defined() != (dt == B200NA_E4M3) || out->value_scale.defined() != (dt == B200NA_E4M3))
+    return false;
+  b200na_kv_cache& c = out->c;
+  c.key = k.data_ptr();
+  c.value = v.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    c.key_stride[i] = k.stride(i);
+    c.value_stride[i] = v.stride(i);
+  }
+  if (dt == B200NA_E4M3) {
+    for (const Tensor* s : {&out->key_scale, &out->value_scale})
+      if (s->scalar_type() != at::kFloat || s->device() != k.device() || s->dim() != 3 ||
+          s->sizes() != k.sizes().slice(0, 3))
+        return false;
+    c.key_scale = out->key_scale.data_ptr<float>();
+    c.value_scale = out->value_scale.data_ptr<float>();
+    for (int i = 0; i < 3; ++i) {
+      c.key_scale_stride[i] = out->key_scale.stride(i);
+      c.value_scale_stride[i] = out->value_scale.stride(i);
+    }
+  }
+  c.pages = k.size(0);
+  c.page_size = (int)k.size(1);
+  c.heads = (int)k.size(2);
+  c.head_dim = (int)k.size(3);
+  c.dtype = dt;
+  return !any_requires_grad({&out->key, &out->value, &out->key_scale, &out->value_scale});
+}
+// A type that the cache is written from, read to or attended in.
+bool cache_takes(const Cache& c, int dt) {
+  return c.c.dtype == B200NA_E4M3 ? dt == B200NA_F32 || is_16bit(dt) : dt == c.c.dtype;
+}
+// int32 [B, pages of a sequence] with contiguous rows
+bool parse_table(PyObject* o, const Cache& c, int64_t batch, Tensor* out) {
+  if (!plain_tensor(o, out) || out->scalar_type() != at::kInt || out->dim() != 2 ||
+      out->device() != c.key.device() || (batch >= 0 && out->size(0) != batch) || out->size(0) > 0x7fffffff ||
+      out->size(1) > 0x7fffffff)
+    return false;
+  if (out->size(1) > 1 && out->stride(1) != 1) *out = out->contiguous();
+  return true;
+}
+// None or int32 [B]
+bool parse_per_sequence(PyObject* o, const Cache& c, int64_t batch, Tensor* out) {
+  if (o == Py_None) return true;
+  if (!plain_tensor(o, out) || out->scalar_type() != at::kInt || out->dim() != 1 || out->size(0) != batch ||
+      out->device() != c.key.device())
+    return false;
+  *out = out->contiguous();
+  return true;
+}
+const int* ints_of(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+// [B, T, heads, D] of the cache's device, contiguous along D
+bool parse_rows(PyObject* o, const Cache& c, Tensor* out) {
+  if (!plain_tensor(o, out) || out->dim() != 4 || out->size(3) != c.c.head_dim ||
+      out->device() != c.key.device() || !cache_takes(c, dtype_code(out->scalar_type())) ||
+      any_requires_grad({out}))
+    return false;
+  for (int i = 0; i < 3; ++i)
+    if (out->size(i) > 0x7fffffff) return false;
+  if (out->size(3) > 1 && out->stride(3) != 1) *out = out->contiguous();
+  return true;
+}
+bool no_shared_elements(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return false;
+  return true;
+}
+
+// kv_cache_write(cache, key, value, page_table, start, counts) -> True
+PyObject* py_kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 6, "kv_cache_write() takes 6 arguments");
+  Cache c;
+  Tensor key, value, table, start, counts;
+  if (!plain_mode() || !parse_cache(a[0], &c) || !parse_rows(a[1], c, &key) || !parse_rows(a[2], c, &value) ||
+      key.sizes() != value.sizes() || key.scalar_type() != value.scalar_type() || key.size(2) != c.c.heads ||
+      !parse_table(a[3], c, key.size(0), &table) || !parse_per_sequence(a[4], c, key.size(0), &start) ||
+      !parse_per_sequence(a[5], c, key.size(0), &counts))
+    Py_RETURN_NONE;
+  const Tensor* const pools[4] = {&c.key, &c.value, &c.key_scale, &c.value_scale};
+  for (const Tensor* t : pools)
+    if (t->defined() && (!no_shared_elements(*t) || (t->is_inference() && !c10::InferenceMode::is_enabled())))
+      Py_RETURN_NONE;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::CUDAGuard guard(key.device());
+    check(lib.kv_cache_write(&c.c, key.data_ptr(), value.data_ptr(), (int)key.size(0), (int)key.size(1),
+                             dtype_code(key.scalar_type()), key.strides().data(), value.strides().data(),
+                             ints_of(table), table.stride(0), (int)table.size(1), ints_of(start),
+                             ints_of(counts), stream_of(key)),
+          "b200na_kv_cache_write");
+    ++launches;
+  }
+  for (const Tensor* t : pools)
+    if (t->defined()) t->unsafeGetTensorImpl()->bump_version();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_cache_read(cache, page_table, length, start, counts, dtype)
+PyObject* py_kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 6, "kv_cache_read() takes 6 arguments");
+  Cache c;
+  Tensor table, start, counts;
+  int length = 0;
+  if (!plain_mode() || !THPDtype_Check(a[5]) || !parse_cache(a[0], &c) || !parse_table(a[1], c, -1, &table) ||
+      !parse_int(a[2], 0, &length) || !parse_per_sequence(a[3], c, table.size(0), &start) ||
+      !parse_per_sequence(a[4], c, table.size(0), &counts))
+    Py_RETURN_NONE;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+  if (!cache_takes(c, dtype_code(type))) Py_RETURN_NONE;
+  Tensor key, value;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(table.device());
+    const std::array<int64_t, 4> shape{table.size(0), length, c.c.heads, c.c.head_dim};
+    key = at::empty(shape, c.key.options().dtype(type));
+    value = at::empty(shape, c.key.options().dtype(type));
+    check(lib.kv_cache_read(&c.c, key.data_ptr(), value.data_ptr(), (int)table.size(0), length,
+                            dtype_code(type), ints_of(table), table.stride(0), (int)table.size(1),
+                            ints_of(start), ints_of(counts), stream_of(table)),
+          "b200na_kv_cache_read");
+    ++launches;
+  }
+  return wrap(key, value, true);
+  END_HANDLE_TH_ERRORS
+}
+
+// na1d_decode(query, cache, page_table, lengths, kernel_size, dilation, scale, return_lse)
+PyObject* py_na1d_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "na1d_decode() takes 8 arguments");
+  Cache c;
+  Tensor q, table, lengths;
+  int kernel = 0, dilation = 1;
+  float scale = 0.f;
+  if (!plain_mode() || !parse_cache(a[1], &c) || !parse_rows(a[0], c, &q) || q.size(2) < c.c.heads ||
+      q.size(2) % c.c.heads || !parse_table(a[2], c, q.size(0), &table) || a[3] == Py_None ||
+      !parse_per_sequence(a[3], c, q.size(0), &lengths) || (a[4] != Py_None && !parse_int(a[4], 2, &kernel)) ||
+      !parse_int(a[5], 1, &dilation) || !parse_scale(a[6], c.c.head_dim, &scale) || std::isinf(scale))
+    Py_RETURN_NONE;
+  const bool want_lse = a[7] == Py_True;
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(q.device());
+    const int B = (int)q.size(0), T = (int)q.size(1), Hq = (int)q.size(2), dt = dtype_code(q.scalar_type());
+    out = at::empty(q.sizes(), q.options());
+    if (want_lse) lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+    const int64_t need =
+        lib.na1d_decode_workspace(B, T, Hq, &c.c, (int)table.size(1), kernel, dilation, dt);
+    if (need < 0) check((int)need, "b200na_na1d_decode_workspace");
+    const Tensor workspace = at::empty({need}, q.options().dtype(at::kByte));
+    check(lib.na1d_decode(q.data_ptr(), q.strides().data(), &c.c, out.data_ptr(),
+                          want_lse ? lse.data_ptr<float>() : nullptr, B, T, Hq, dt, ints_of(table),
+                          table.stride(0), (int)table.size(1), ints_of(lengths), kernel, dilation, scale,
+                          workspace.data_ptr(), stream_of(q)),
+          "b200na_na1d_decode");
+    launches += 2;
+  }
+  return wrap(out, lse, want_lse);
+  END_HANDLE_TH_ERRORS
+}
+
 // tiles(backward, shape, kernel, stride, dilation, is_causal[, extra]) -> (q tile, kv tile); with
 // `extra` (whether there are extra tokens) the plan of the entries for views
 PyObject* py_tiles(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -1223,6 +1592,10 @@ PyMethodDef methods[] = {
     {"na", (PyCFunction)(void*)py_na, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void*)py_attention, METH_FASTCALL, nullptr},
     {"layer", (PyCFunction)(void*)py_layer, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void*)py_rotary, METH_FASTCALL, nullptr},
+    {"kv_cache_write", (PyCFunction)(void*)py_kv_cache_write, METH_FASTCALL, nullptr},
+    {"kv_cache_read", (PyCFunction)(void*)py_kv_cache_read, METH_FASTCALL, nullptr},
+    {"na1d_decode", (PyCFunction)(void*)py_na1d_decode, METH_FASTCALL, nullptr},
     {"tiles", (PyCFunction)(void*)py_tiles, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "torch_binding", nullptr, -1, methods,

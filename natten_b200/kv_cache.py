@@ -12,9 +12,9 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from . import ops
+from . import _native, ops
 from .checks import _dim_arg
-from .functional import _require_cuda, _wants_grad
+from .functional import _native_eligible, _require_cuda, _wants_grad
 
 COMPUTE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 CACHE_DTYPES = COMPUTE_DTYPES + (torch.float8_e4m3fn,)
@@ -125,6 +125,9 @@ def kv_cache_write(cache: KVCache, key: Tensor, value: Tensor, page_table: Tenso
     Positions that are negative, behind the table, or on a table entry outside ``[0, pages)`` are dropped.
     The slots of one call must be different ones: of two tokens on the same slot, which one (or a mixture)
     is left is undefined."""
+    if (_native_eligible()
+            and _native.kv_cache_write(cache, key, value, page_table, start, counts) is not None):
+        return
     _check_cache(cache)
     _check_rows(cache, key=key, value=value)
     if key.shape != value.shape or key.shape[2] != cache.key.shape[2] or key.dtype != value.dtype:
@@ -150,9 +153,13 @@ def kv_cache_read(cache: KVCache, page_table: Tensor, length: int, start: Option
     Row t of sequence b is the token at ``start[b] + t`` (``t`` without ``start``); rows ``t >= counts[b]``
     and tokens that are on no page are zeros. ``dtype`` is the cache's, or fp32, fp16 or bf16 for an 8-bit
     cache (default bf16)."""
-    _check_cache(cache)
     if dtype is None:
         dtype = torch.bfloat16 if cache.key.dtype == torch.float8_e4m3fn else cache.key.dtype
+    if _native_eligible():
+        result = _native.kv_cache_read(cache, page_table, length, start, counts, dtype)
+        if result is not None:
+            return result
+    _check_cache(cache)
     _check_dtype(cache, dtype, "dtype")
     if not isinstance(length, int) or isinstance(length, bool) or not 0 <= length < 2 ** 31:
         raise ValueError(f"`length` must be a number of tokens, got {length!r}.")
@@ -181,6 +188,11 @@ def na1d_decode(query: Tensor, cache: KVCache, page_table: Tensor, lengths: Tens
 
     The cache has the query's data type or is an 8-bit one. Returns the output in the query's type, with
     ``return_lse`` also the logsumexp (fp32 ``[batch, tokens, heads]``), as `merge_attentions` takes them."""
+    if _native_eligible():
+        result = _native.na1d_decode(query, cache, page_table, lengths, kernel_size, dilation, scale,
+                                     bool(return_lse))
+        if result is not None:
+            return result
     _check_cache(cache)
     _check_rows(cache, query=query)
     heads, heads_kv = query.shape[2], cache.key.shape[2]

@@ -7,8 +7,8 @@ from typing import Any, Optional, Sequence, Tuple, Union
 import torch
 from torch import Tensor
 
-from . import ops
-from .functional import _require_cuda
+from . import _native, ops
+from .functional import _native_eligible, _require_cuda
 
 ROTARY_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_HEAD_DIM = 256
@@ -64,6 +64,10 @@ def rotary(query: Tensor, key: Optional[Tensor] = None, axis_dims: Optional[Sequ
 
     Returns new contiguous tensors: the query alone when there is no key, else (query, key). fp32, fp16
     and bf16, head dims up to 256; differentiable in query and key, also twice."""
+    if _native_eligible():
+        result = _native.rotary(query, key, axis_dims, theta, positions, origin, position_scale, interleaved)
+        if result is not None:
+            return result
     for name, t in (("Query", query), ("Key", key)):
         if t is None:
             continue

@@ -313,3 +313,28 @@ def test_a_run_of_them_together(cache_dtype):
     key, value = nb.kv_cache_read(cache, table, N)
     if cache_dtype == torch.bfloat16:
         assert torch.equal(key, kr) and torch.equal(value, v)
+
+
+def test_native_front_and_registered_operators_give_the_same(monkeypatch):
+    """The call from C++ and the one through the registered operators, and the versions of what they
+    write."""
+    import natten_b200.kv_cache as module
+    for dtype, cache_dtype in TYPES:
+        q, cache, table, n = _state(dtype, cache_dtype, [120, 64], 3, 4, 2, 64, 16)
+        k = torch.randn(2, 3, 2, 64, device="cuda").to(dtype)
+        got = []
+        for native in (True, False):
+            monkeypatch.setattr(module, "_native_eligible", lambda native=native: native)
+            c = nb.KVCache(*(None if t is None else t.clone() for t in cache))
+            version = c.key._version
+            nb.kv_cache_write(c, k, k, table, n - 3, counts=torch.full_like(n, 2))
+            assert c.key._version > version
+            got.append((*c[:2], *nb.kv_cache_read(c, table, 130, dtype=dtype),
+                        *nb.na1d_decode(q, c, table, n, 50, return_lse=True), nb.na1d_decode(q, c, table, n)))
+        for x, y in zip(*got):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    before = L.launches
+    monkeypatch.setattr(module, "_native_eligible", lambda: True)
+    nb.na1d_decode(q, c, table, n)
+    nb.kv_cache_read(c, table, 5, dtype=dtype)
+    assert L.launches == before + 3

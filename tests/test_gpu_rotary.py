@@ -221,3 +221,29 @@ def test_op_and_compile():
     (h,) = torch.autograd.grad(f(leaf, k)[0].sum(), leaf)
     assert torch.equal(g, h)
     assert L.device_status() == 0
+
+
+def test_native_front_and_registered_operators_give_the_same(monkeypatch):
+    import natten_b200.positions as module
+    torch.manual_seed(10)
+    q = torch.randn(2, 5, 6, 4, 64).bfloat16().cuda().requires_grad_()
+    k = torch.randn(2, 5, 6, 2, 64).bfloat16().cuda().requires_grad_()
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    at = torch.randint(0, 99, (1, 5, 6, 3), device="cuda")
+    for kw in ({}, {"positions": at}, {"axis_dims": [8, 24], "theta": (10, 1e5), "origin": (3, -1),
+                                       "position_scale": (2, 0.5), "interleaved": True}):
+        got = []
+        for native in (True, False):
+            monkeypatch.setattr(module, "_native_eligible", lambda native=native: native)
+            a, b = nb.rotary(q, k, **kw)
+            got.append((a, b, nb.rotary(q.detach(), **kw), *torch.autograd.grad((a, b), (q, k), (dq, dk)),
+                        torch.autograd.grad(nb.rotary(q, k.detach(), **kw)[0], q, dq)[0],
+                        torch.autograd.grad(nb.rotary(q.detach(), k, **kw)[1], k, dk)[0]))
+        for x, y in zip(*got):
+            assert torch.equal(x, y)
+    # the gradients of both operands in one launch
+    monkeypatch.setattr(module, "_native_eligible", lambda: True)
+    a, b = nb.rotary(q, k)
+    before = L.launches
+    torch.autograd.grad((a, b), (q, k), (dq, dk))
+    assert L.launches == before + 1
