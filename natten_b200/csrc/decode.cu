@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 #pragma unroll
       for (int x = 0; x < kRows; ++x) s[x] = 0.f;
       if (there)
+#pragma unroll 4
         for (int d = 0; d < a.D; d += kVec) {
           const Elements<P, kVec> kk = *reinterpret_cast<const Elements<P, kVec>*>(k + d);
 #pragma unroll
@@ -345,23 +346,29 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
         for (int e = 0; e < kD32; ++e) acc[x][e] *= keep;
         s[x] *= v_scale;
       }
+      // kAhead value rows are under way together
+      constexpr int kAhead = kD32 > 4 ? 4 : 8;
       const int count = min(32, end - i0);
-      for (int key = 0; key < count; ++key) {
-        const int64_t off = __shfl_sync(0xffffffffu, v_at, key);
-        const bool has = __shfl_sync(0xffffffffu, (int)there, key);
-        if (!has) continue;
-        const P* v = static_cast<const P*>(a.value.base) + off;
-        float vv[kD32];
+      for (int key0 = 0; key0 < count; key0 += kAhead) {
+        P vv[kAhead][kD32];
 #pragma unroll
-        for (int e = 0; e < kD32; ++e) vv[e] = lane + 32 * e < a.D ? as_float(v[lane + 32 * e]) : 0.f;
+        for (int z = 0; z < kAhead; ++z) {
+          const int64_t off = __shfl_sync(0xffffffffu, v_at, key0 + z);     // (0, and no row's, behind the last)
+          const P* v = static_cast<const P*>(a.value.base) + off;
+          const bool has = key0 + z < count && __shfl_sync(0xffffffffu, (int)there, key0 + z);
 #pragma unroll
-        for (int x = 0; x < kRows; ++x) {
-          const float p = __shfl_sync(0xffffffffu, s[x], key);
-          // a NaN or an infinity stays with the rows that attend its token
-          if (seen[x] >> key & 1)
-#pragma unroll
-            for (int e = 0; e < kD32; ++e) acc[x][e] += p * vv[e];
+          for (int e = 0; e < kD32; ++e) vv[z][e] = has && lane + 32 * e < a.D ? v[lane + 32 * e] : P(0.f);
         }
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z)
+#pragma unroll
+          for (int x = 0; x < kRows; ++x) {
+            const float p = __shfl_sync(0xffffffffu, s[x], key0 + z);
+            // a NaN or an infinity stays with the rows that attend its token
+            if (seen[x] >> (key0 + z) & 1)
+#pragma unroll
+              for (int e = 0; e < kD32; ++e) acc[x][e] += p * as_float(vv[z][e]);
+          }
       }
     }
 #pragma unroll
@@ -392,14 +399,12 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 template <class T> struct Half2Of;
 template <> struct Half2Of<__half> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
+    return bits_as<uint32_t>(__floats2half2_rn(x, y));
   }
 };
 template <> struct Half2Of<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
+    return bits_as<uint32_t>(__floats2bfloat162_rn(x, y));
   }
 };
 
@@ -635,7 +640,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) q[k][x + 2 * e] = *reinterpret_cast<const uint32_t*>(&v[k][e]);
+          for (int e = 0; e < 2; ++e) q[k][x + 2 * e] = bits_as<uint32_t>(v[k][e]);
       }
     }
     // Tiles whose first key lies in [safe_from, safe_to] are attended whole, or not, by all rows alike.
@@ -814,8 +819,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
                 if (!(odd >> (8 * kElem * e) & 1)) continue;
                 float y = __int_as_float(0x7fc00000);
                 if (!k8) {
-                  const uint16_t bits = word >> (16 * e);
-                  y = as_float(*reinterpret_cast<const T*>(&bits));
+                  y = as_float(bits_as<T>((uint16_t)(word >> (16 * e))));
                 }
                 acc[k8 ? 2 * i + (e & 1) : i][2 * x + (k8 ? e >> 1 : e)] += y;
               }

@@ -3,15 +3,15 @@
 // Both are streams of rows (one token's channels of one head): a row is read once and written once,
 // keys and values in one launch. A group of lanes holds a whole row in registers, 16 bytes a lane and
 // access, so the largest magnitude of a row (for its 8-bit scale) is a few shuffles away and the row is
-// not read again.
-#include <type_traits>
-
+// not read again. A block works on consecutive tokens of one sequence, so that a sequence's start and
+// count are read once a block and places need 32-bit arithmetic only; a thread has kRows rows in flight.
 #include "paged.cuh"
 
 namespace b200na {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRows = 4;         // rows of keys and of values that a thread has in flight
 
 struct MoveArgs {
   PagedPool pool[2];             // keys, values
@@ -21,111 +21,165 @@ struct MoveArgs {
   const int* start;
   const int* counts;
   int B, T, heads, D;
+  int tokens;                    // of a block
+  int tiles;                     // blocks of a sequence
 };
 
 // Lanes per row: a power of two that holds D / kVec accesses, 32 at most (then several each).
 template <class T, class P, int kVec, bool kWrite>
-__global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes) {
+__global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes_log2) {
   constexpr int kMost = kVec >= 8 ? 1 : kVec >= 4 ? 2 : 8;    // accesses a lane makes of one row, D <= 256
+  constexpr int kAtOnce = kMost == 8 ? 1 : kRows / (kMost * (int)sizeof(T) * kVec > 16 ? 2 : 1);
   constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t per_step = (int64_t)gridDim.x * (kThreads / lanes);
-  const int64_t rows = (int64_t)a.B * a.T * a.heads;
-  const int accesses = a.D / kVec;
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int group = threadIdx.x >> lanes_log2, groups = kThreads >> lanes_log2;
+  const int b = blockIdx.x / a.tiles, t0 = (blockIdx.x - b * a.tiles) * a.tokens;
+  const int count = a.counts ? min(a.counts[b], a.T) : a.T;          // tokens that are moved
+  const int here = min(a.tokens, (kWrite ? count : a.T) - t0);       // rows of tokens t0 + [0, here)
+  if (here <= 0) return;
+  const int64_t start = a.start ? a.start[b] : 0;
+  const int accesses = a.D / kVec, rows = here * a.heads;
   // (every lane of a warp takes part in every round: the shuffles below need them all)
-  const int64_t first = (int64_t)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
-  for (int64_t round = first - threadIdx.x / lanes; round < rows; round += per_step) {
-    const int64_t row = round + threadIdx.x / lanes;
-    bool live = row < rows;
-    const int64_t token = live ? row / a.heads : 0;
-    const int h = live ? (int)(row - token * a.heads) : 0;
-    const int b = (int)(token / a.T), t = (int)(token - (int64_t)b * a.T);
-    const bool inside = live && (!a.counts || t < a.counts[b]);
-    int64_t page = -1;
-    int slot = 0;
-    if (inside) {
-      const int64_t p = (a.start ? (int64_t)a.start[b] : 0) + t;
-      int64_t index;
-      if (p >= 0) {
-        a.table.split(p, &index, &slot);
-        page = a.table.page_of(b, index);
+  for (int row0 = 0; row0 < rows; row0 += groups * kAtOnce) {
+    using In = Raw<T, kVec>;
+    using Cached = Raw<P, kVec>;
+    In x[kAtOnce][2][kMost];
+    bool live[kAtOnce];
+    int t[kAtOnce], h[kAtOnce];
+    int64_t page[kAtOnce];
+    int slot[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int row = row0 + u * groups + group;
+      live[u] = row < rows;
+      const int tt = live[u] ? (int)((uint32_t)row / (uint32_t)a.heads) : 0;
+      h[u] = live[u] ? row - tt * a.heads : 0;
+      t[u] = t0 + tt;
+    }
+    if (kWrite) {
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const T* data = static_cast<const T*>(a.data[w]) + b * a.batch[w] + t[u] * a.token[w] + h[u] * a.head[w];
+#pragma unroll
+          for (int i = 0; i < kMost; ++i)
+            if (live[u] && lane + (i << lanes_log2) < accesses)
+              x[u][w][i] = *reinterpret_cast<const In*>(data + (lane + (i << lanes_log2)) * kVec);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      page[u] = -1;
+      slot[u] = 0;
+      const int64_t p = start + t[u];
+      if (live[u] && t[u] < count && p >= 0) {
+        int64_t index;
+        a.table.split(p, &index, &slot[u]);
+        page[u] = a.table.page_of(b, index);
       }
     }
-    if (kWrite) live = page >= 0;
+    if (kWrite) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const PagedPool& pool = a.pool[w];
-      P* cached = static_cast<P*>(pool.base) + page * pool.page + (int64_t)slot * pool.token + h * pool.head;
-      T* data = static_cast<T*>(a.data[w]) + b * a.batch[w] + (int64_t)t * a.token[w] + h * a.head[w];
-      float* scale_at = kScaled ? pool.scale + page * pool.s_page + (int64_t)slot * pool.s_token + h * pool.s_head
-                                : nullptr;
-      if (kWrite) {
-        Elements<T, kVec> x[kMost];
-        float most = 0.f;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const bool to = page[u] >= 0;
+        float inverse[2] = {1.f, 1.f};
+        if constexpr (kScaled) {
+          float most[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) {
-          const int at = lane + i * lanes;
-          if (live && at < accesses) {
-            x[i] = *reinterpret_cast<const Elements<T, kVec>*>(data + at * kVec);
-            if (kScaled) {
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-              for (int e = 0; e < kVec; ++e) {
-                const float m = fabsf(as_float(x[i].v[e]));
-                most = fmaxf(most, m < INFINITY ? m : INFINITY);   // infinity also for a NaN
+            for (int i = 0; i < kMost; ++i)
+              if (live[u] && lane + (i << lanes_log2) < accesses) {
+                float f[kVec];
+                to_floats<T, kVec>(x[u][w][i], f);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                  const float m = fabsf(f[e]);
+                  most[w] = fmaxf(most[w], m < INFINITY ? m : INFINITY);   // infinity also for a NaN
+                }
               }
-            }
+          for (int o = lanes / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) most[w] = fmaxf(most[w], __shfl_xor_sync(0xffffffffu, most[w], o));
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            // not finite: the whole row reads back as NaN
+            const float scale = most[w] < INFINITY ? fmaxf(__fdiv_rn(most[w], kE4m3Max), kSmallestScale)
+                                                   : __int_as_float(0x7fc00000);
+            inverse[w] = __frcp_rn(scale);
+            const PagedPool& pool = a.pool[w];
+            if (to && lane == 0)
+              pool.scale[page[u] * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head] = scale;
           }
         }
-        float inverse = 1.f;
-        if (kScaled) {
-          for (int o = lanes / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          // not finite: the whole row reads back as NaN
-          const float scale = most < INFINITY ? fmaxf(__fdiv_rn(most, kE4m3Max), kSmallestScale)
-                                              : __int_as_float(0x7fc00000);
-          inverse = __frcp_rn(scale);
-          if (live && lane == 0) *scale_at = scale;
-        }
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) {
-          const int at = lane + i * lanes;
-          if (live && at < accesses) {
-            Elements<P, kVec> y;
+        for (int w = 0; w < 2; ++w) {
+          const PagedPool& pool = a.pool[w];
+          P* const cached = static_cast<P*>(pool.base) + (to ? page[u] * pool.page + slot[u] * pool.token + h[u] * pool.head : 0);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-              if constexpr (kScaled) y.v[e] = from_float<P>(as_float(x[i].v[e]) * inverse);
-              else y.v[e] = x[i].v[e];
-            }
-            *reinterpret_cast<Elements<P, kVec>*>(cached + at * kVec) = y;
-          }
-        }
-      } else {
-        const float scale = kScaled && page >= 0 ? *scale_at : 0.f;
+          for (int i = 0; i < kMost; ++i)
+            if (to && lane + (i << lanes_log2) < accesses) {
+              Cached y;
+              if constexpr (kScaled) {
+                float f[kVec];
+                to_floats<T, kVec>(x[u][w][i], f);
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) {
-          const int at = lane + i * lanes;
-          if (live && at < accesses) {
-            Elements<T, kVec> y;
-            if (page >= 0) {
-              const Elements<P, kVec> x = *reinterpret_cast<const Elements<P, kVec>*>(cached + at * kVec);
-#pragma unroll
-              for (int e = 0; e < kVec; ++e) {
-                if constexpr (kScaled) y.v[e] = from_float<T>(as_float(x.v[e]) * scale);
-                else y.v[e] = x.v[e];
+                for (int e = 0; e < kVec; ++e) f[e] *= inverse[w];
+                y = from_floats<P, kVec>(f);
+              } else {
+                y = x[u][w][i];
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < kVec; ++e) y.v[e] = from_float<T>(0.f);
+              *reinterpret_cast<Cached*>(cached + (lane + (i << lanes_log2)) * kVec) = y;
             }
-            *reinterpret_cast<Elements<T, kVec>*>(data + at * kVec) = y;
-          }
         }
       }
+    } else {
+      Cached y[kAtOnce][2][kMost];
+      float scale[kAtOnce][2];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const PagedPool& pool = a.pool[w];
+          const bool from = page[u] >= 0;
+          scale[u][w] = 0.f;
+          if (kScaled && from)
+            scale[u][w] = pool.scale[page[u] * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head];
+          const P* const cached = static_cast<const P*>(pool.base) + (from ? page[u] * pool.page + slot[u] * pool.token + h[u] * pool.head : 0);
+#pragma unroll
+          for (int i = 0; i < kMost; ++i) {
+            y[u][w][i] = Cached{};
+            if (from && lane + (i << lanes_log2) < accesses)
+              y[u][w][i] = *reinterpret_cast<const Cached*>(cached + (lane + (i << lanes_log2)) * kVec);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          T* const data = static_cast<T*>(a.data[w]) + b * a.batch[w] + t[u] * a.token[w] + h[u] * a.head[w];
+#pragma unroll
+          for (int i = 0; i < kMost; ++i)
+            if (live[u] && lane + (i << lanes_log2) < accesses) {
+              if constexpr (kScaled) {
+                float f[kVec];
+                to_floats<P, kVec>(y[u][w][i], f);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) f[e] *= scale[u][w];
+                x[u][w][i] = from_floats<T, kVec>(f);
+              } else {
+                x[u][w][i] = y[u][w][i];
+              }
+              *reinterpret_cast<In*>(data + (lane + (i << lanes_log2)) * kVec) = x[u][w][i];
+            }
+        }
     }
   }
 }
 
 template <class T, class P, bool kWrite>
-int launch(const MoveArgs& a, cudaStream_t stream) {
+int launch(MoveArgs a, cudaStream_t stream) {
   constexpr int kWide = 16 / (int)sizeof(T);
   // whole 16-byte accesses where sizes, strides and addresses of both sides allow
   bool wide = a.D % kWide == 0;
@@ -136,16 +190,16 @@ int launch(const MoveArgs& a, cudaStream_t stream) {
            (a.batch[w] | a.token[w] | a.head[w] | p.page | p.token | p.head) % kWide == 0;
   }
   const int accesses = wide ? a.D / kWide : a.D;
-  int lanes = 1;
-  while (lanes < 32 && lanes < accesses) lanes *= 2;
-  int sms = 0;
-  const int rc = sm_count_of_current_device(&sms);
-  if (rc != B200NA_OK) return rc;
-  const int64_t rows = (int64_t)a.B * a.T * a.heads, per_block = kThreads / lanes;
-  int64_t blocks = (rows + per_block - 1) / per_block;
-  if (blocks > (int64_t)sms * 64) blocks = (int64_t)sms * 64;
-  if (wide) move_kernel<T, P, kWide, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes);
-  else move_kernel<T, P, 1, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes);
+  int lanes_log2 = 0;
+  while (lanes_log2 < 5 && (1 << lanes_log2) < accesses) ++lanes_log2;
+  // tokens of a block: one round of its threads' rows, at least one token
+  const int rows = (kThreads >> lanes_log2) * kRows;
+  a.tokens = rows > a.heads ? rows / a.heads : 1;
+  a.tiles = (a.T + a.tokens - 1) / a.tokens;
+  const int64_t blocks = (int64_t)a.B * a.tiles;
+  if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
+  if (wide) move_kernel<T, P, kWide, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes_log2);
+  else move_kernel<T, P, 1, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes_log2);
   B200NA_CUDA_TRY(cudaGetLastError());
   return B200NA_OK;
 }

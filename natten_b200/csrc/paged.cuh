@@ -6,6 +6,9 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <cstring>
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200na {
@@ -106,5 +109,57 @@ template <class T, int kN>
 struct alignas(sizeof(T) * kN) Elements {
   T v[kN];
 };
+
+// The bits of `x` as another type of the same size.
+template <class To, class From> __device__ __forceinline__ To bits_as(const From& x) {
+  static_assert(sizeof(To) == sizeof(From), "sizes differ");
+  To y;
+  memcpy(&y, &x, sizeof(To));
+  return y;
+}
+
+// kBytes as one access.
+template <int kBytes> struct RawOf;
+template <> struct RawOf<1> { using type = uint8_t; };
+template <> struct RawOf<2> { using type = uint16_t; };
+template <> struct RawOf<4> { using type = uint32_t; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<16> { using type = uint4; };
+template <class T, int kN> using Raw = typename RawOf<(int)sizeof(T) * kN>::type;
+
+// kN elements out of their bits and back. 8 bits: two values an instruction.
+template <class T, int kN> __device__ __forceinline__ void to_floats(const Raw<T, kN>& bits, float (&y)[kN]) {
+  if constexpr (std::is_same<T, __nv_fp8_e4m3>::value && kN % 2 == 0) {
+    __nv_fp8x2_storage_t x[kN / 2];
+    memcpy(x, &bits, kN);
+#pragma unroll
+    for (int e = 0; e < kN / 2; ++e) {
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(x[e], __NV_E4M3)));
+      y[2 * e] = f.x;
+      y[2 * e + 1] = f.y;
+    }
+  } else {
+    T x[kN];
+    memcpy(x, &bits, sizeof(x));
+#pragma unroll
+    for (int e = 0; e < kN; ++e) y[e] = as_float(x[e]);
+  }
+}
+template <class T, int kN> __device__ __forceinline__ Raw<T, kN> from_floats(const float (&x)[kN]) {
+  Raw<T, kN> bits;
+  if constexpr (std::is_same<T, __nv_fp8_e4m3>::value && kN % 2 == 0) {
+    __nv_fp8x2_storage_t y[kN / 2];
+#pragma unroll
+    for (int e = 0; e < kN / 2; ++e)
+      y[e] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * e], x[2 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+    memcpy(&bits, y, kN);
+  } else {
+    T y[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) y[e] = from_float<T>(x[e]);
+    memcpy(&bits, y, sizeof(y));
+  }
+  return bits;
+}
 
 }  // namespace b200na

@@ -7,18 +7,17 @@
 // position * (f / 2 pi) is formed and reduced in fp64 and only the fraction of a turn goes to the fp32
 // sincospi. A block works the angles of its tokens out once, into shared memory, and uses them for all
 // heads of queries and keys. The rest is a stream: every element is read once and written once.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <cmath>
 
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace b200na {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;   // head_dim <= 256
+constexpr int kMostTokens = 16;  // of a block
+constexpr int kUnroll = 2;
 
 struct RotaryArgs {
   const void* in[2];
@@ -27,7 +26,7 @@ struct RotaryArgs {
   int heads[2];
   int ndim, B, D, axes;
   int shape[3];
-  int64_t tokens;                // of all batch entries
+  int64_t tokens, batch_tokens;  // of all batch entries, of one
   int first_pair[4];             // pairs before axis a
   double origin[3];
   double turns[kMaxPairs];       // frequency of each pair in turns per position, negated for the inverse
@@ -35,110 +34,130 @@ struct RotaryArgs {
   int position_type, positions_batched;
 };
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
-template <class T, int kN>
-struct alignas(sizeof(T) * kN) Pack {
-  T v[kN];
-};
-
 // kVec: pairs that a thread turns at once. Halves: kVec channels of each half, interleaved: 2 kVec
-// neighbours.
+// neighbours. A thread keeps its column of the rows, so that what depends on it is worked out once.
 template <class T, int kVec, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a,
                                                           int block_tokens) {
-  extern __shared__ float2 cs[];                              // [block_tokens][pairs]
-  __shared__ int64_t in_at[2][16], out_at[2][16];             // element offsets of the tokens' first head
-  const int pairs = a.first_pair[a.axes];
+  extern __shared__ __align__(16) float cs[];                 // [block_tokens][cosines, sines][stride]
+  __shared__ int64_t in_at[2][kMostTokens], out_at[2][kMostTokens];   // offsets of the tokens' first head
+  __shared__ double place[kMostTokens][3];
+  const int pairs = a.first_pair[a.axes], stride = (pairs + 3) / 4 * 4;
   const int64_t token0 = (int64_t)blockIdx.x * block_tokens;
   const int count = (int)(a.tokens - token0 < block_tokens ? a.tokens - token0 : block_tokens);
-  const int64_t per_batch = a.tokens / a.B;
 
-  for (int i = threadIdx.x; i < count * pairs; i += kThreads) {
-    const int tt = i / pairs, pair = i - tt * pairs;
-    int axis = 0;
-    while (axis + 1 < a.axes && pair >= a.first_pair[axis + 1]) ++axis;
-    const int64_t token = token0 + tt;
-    double at;
-    if (a.positions) {
-      const int64_t row = a.positions_batched ? token : token % per_batch;
-      const int64_t e = row * a.axes + axis;
-      at = a.position_type == 0   ? (double)static_cast<const int*>(a.positions)[e]
-           : a.position_type == 1 ? (double)static_cast<const int64_t*>(a.positions)[e]
-                                  : (double)static_cast<const float*>(a.positions)[e];
-    } else {
-      int64_t rest = token % per_batch;
-      int x = 0;
-      for (int d = a.ndim - 1; d >= axis; --d) {
-        x = (int)(rest % a.shape[d]);
-        rest /= a.shape[d];
-      }
-      at = a.origin[axis] + x;
-    }
-    const double turn = at * a.turns[pair];
-    float s, c;
-    sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
-    cs[i] = make_float2(c, s);
-  }
   if ((int)threadIdx.x < count) {
-    const int64_t token = token0 + threadIdx.x, b = token / per_batch;
-    int64_t rest = token - b * per_batch;
-    for (int w = 0; w < 2; ++w) {
-      int64_t off = b * a.stride[w][0], r = rest;
-      for (int d = a.ndim - 1; d >= 0; --d) {
-        off += (r % a.shape[d]) * a.stride[w][1 + d];
-        r /= a.shape[d];
+    const int tt = threadIdx.x;
+    const int64_t token = token0 + tt, b = token / a.batch_tokens, rest = token - b * a.batch_tokens;
+    int64_t off[2] = {b * a.stride[0][0], b * a.stride[1][0]};
+    uint64_t r = rest;
+    for (int d = a.ndim - 1; d >= 0; --d) {
+      uint64_t up = 0;
+      uint32_t x = (uint32_t)r;
+      if (d > 0) {
+        up = r >> 32 ? r / a.shape[d] : (uint32_t)r / (uint32_t)a.shape[d];
+        x = (uint32_t)(r - up * a.shape[d]);
       }
-      in_at[w][threadIdx.x] = off;
-      out_at[w][threadIdx.x] = token * a.heads[w] * a.D;
+      r = up;
+      off[0] += x * a.stride[0][1 + d];
+      off[1] += x * a.stride[1][1 + d];
+      if (!a.positions) place[tt][d] = a.origin[d] + (double)x;
+    }
+    if (a.positions) {
+      const int64_t e = (a.positions_batched ? token : rest) * a.axes;
+      for (int axis = 0; axis < a.axes; ++axis)
+        place[tt][axis] = a.position_type == 0   ? (double)static_cast<const int*>(a.positions)[e + axis]
+                          : a.position_type == 1 ? (double)static_cast<const int64_t*>(a.positions)[e + axis]
+                                                 : (double)static_cast<const float*>(a.positions)[e + axis];
+    }
+    for (int w = 0; w < 2; ++w) {
+      in_at[w][tt] = off[w];
+      out_at[w][tt] = token * a.heads[w] * a.D;
     }
   }
   __syncthreads();
+  for (int i = threadIdx.x; i < count * pairs; i += kThreads) {
+    const int tt = i / pairs, pair = i - tt * pairs;
+    const int axis = (pair >= a.first_pair[1] && a.axes > 1) + (pair >= a.first_pair[2] && a.axes > 2);
+    const double turn = place[tt][axis] * a.turns[pair];
+    float s, c;
+    sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
+    cs[2 * tt * stride + pair] = c;
+    cs[(2 * tt + 1) * stride + pair] = s;
+  }
+  __syncthreads();
 
-  const int heads = a.heads[0] + a.heads[1];
-  const int rows = count * heads;
-  const int chunks = pairs / kVec;          // of the turned channels of a row
-  for (int i = threadIdx.x; i < rows * chunks; i += kThreads) {
-    const int row = i / chunks, pair = (i - row * chunks) * kVec;
-    const int tt = row / heads;
-    int h = row - tt * heads;
-    const int w = h >= a.heads[0];
-    if (w) h -= a.heads[0];
-    const T* in = static_cast<const T*>(a.in[w]) + in_at[w][tt] + h * a.stride[w][a.ndim + 1];
-    T* out = static_cast<T*>(a.out[w]) + out_at[w][tt] + (int64_t)h * a.D;
-    const float2* t = cs + tt * pairs + pair;
-    if (kInterleaved && kVec > 1) {
-      Pack<T, 2 * kVec> x = *reinterpret_cast<const Pack<T, 2 * kVec>*>(in + 2 * pair);
+  const int heads = a.heads[0] + a.heads[1], rows = count * heads;
+  const int chunks = pairs / kVec, at_once = chunks > 0 ? kThreads / chunks : 0;
+  const int group = chunks > 0 ? threadIdx.x / chunks : 0;
+  if (group < at_once) {
+    const int pair = (threadIdx.x - group * chunks) * kVec;
+    const int axis = (pair >= a.first_pair[1] && a.axes > 1) + (pair >= a.first_pair[2] && a.axes > 2);
+    const int half = kInterleaved ? 1 : a.first_pair[axis + 1] - a.first_pair[axis];
+    const int lo = kInterleaved ? 2 * pair : a.first_pair[axis] + pair;     // 2 first + (pair - first)
+    const int64_t head_stride[2] = {a.stride[0][a.ndim + 1], a.stride[1][a.ndim + 1]};
+    int tt = group / heads, h = group - tt * heads;
+    for (int row = group; row < rows; row += kUnroll * at_once) {
+      // kUnroll rows at a time: their loads are under way together
+      Elements<T, kVec> x[kUnroll], y[kUnroll];
+      T* dst[kUnroll];
+      const float* table[kUnroll];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const float u = to_f(x.v[2 * e]), v = to_f(x.v[2 * e + 1]);
-        x.v[2 * e] = from_f<T>(u * t[e].x - v * t[e].y);
-        x.v[2 * e + 1] = from_f<T>(u * t[e].y + v * t[e].x);
-      }
-      *reinterpret_cast<Pack<T, 2 * kVec>*>(out + 2 * pair) = x;
-    } else {
-      int axis = 0;
-      while (axis + 1 < a.axes && pair >= a.first_pair[axis + 1]) ++axis;
-      const int half = kInterleaved ? 1 : a.first_pair[axis + 1] - a.first_pair[axis];
-      const int lo = kInterleaved ? 2 * pair : a.first_pair[axis] + pair;   // 2 first + (pair - first)
-      Pack<T, kVec> x = *reinterpret_cast<const Pack<T, kVec>*>(in + lo);
-      Pack<T, kVec> y = *reinterpret_cast<const Pack<T, kVec>*>(in + lo + half);
+      for (int u = 0; u < kUnroll; ++u) {
+        dst[u] = nullptr;
+        if (row + u * at_once < rows) {
+          const int w = h >= a.heads[0], hh = w ? h - a.heads[0] : h;
+          const T* const src = static_cast<const T*>(a.in[w]) + in_at[w][tt] + hh * head_stride[w] + lo;
+          dst[u] = static_cast<T*>(a.out[w]) + out_at[w][tt] + hh * a.D + lo;
+          table[u] = cs + 2 * tt * stride + pair;
+          if constexpr (kInterleaved && kVec > 1) {
+            const Elements<T, 2 * kVec> both = *reinterpret_cast<const Elements<T, 2 * kVec>*>(src);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const float u = to_f(x.v[e]), v = to_f(y.v[e]);
-        x.v[e] = from_f<T>(u * t[e].x - v * t[e].y);
-        y.v[e] = from_f<T>(u * t[e].y + v * t[e].x);
+            for (int e = 0; e < kVec; ++e) {
+              x[u].v[e] = both.v[2 * e];
+              y[u].v[e] = both.v[2 * e + 1];
+            }
+          } else {
+            x[u] = *reinterpret_cast<const Elements<T, kVec>*>(src);
+            y[u] = *reinterpret_cast<const Elements<T, kVec>*>(src + half);
+          }
+        }
+        h += at_once;
+        while (h >= heads) {
+          h -= heads;
+          ++tt;
+        }
       }
-      *reinterpret_cast<Pack<T, kVec>*>(out + lo) = x;
-      *reinterpret_cast<Pack<T, kVec>*>(out + lo + half) = y;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (!dst[u]) continue;
+        alignas(16) float cosine[kVec], sine[kVec];
+        constexpr int kLoad = kVec < 4 ? kVec : 4;
+#pragma unroll
+        for (int e = 0; e < kVec; e += kLoad) {
+          *reinterpret_cast<Elements<float, kLoad>*>(cosine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(table[u] + e);
+          *reinterpret_cast<Elements<float, kLoad>*>(sine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(table[u] + stride + e);
+        }
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float c = cosine[e], s = sine[e];
+          const float p = as_float(x[u].v[e]), q = as_float(y[u].v[e]);
+          x[u].v[e] = from_float<T>(p * c - q * s);
+          y[u].v[e] = from_float<T>(p * s + q * c);
+        }
+        if constexpr (kInterleaved && kVec > 1) {
+          Elements<T, 2 * kVec> both;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) {
+            both.v[2 * e] = x[u].v[e];
+            both.v[2 * e + 1] = y[u].v[e];
+          }
+          *reinterpret_cast<Elements<T, 2 * kVec>*>(dst[u]) = both;
+        } else {
+          *reinterpret_cast<Elements<T, kVec>*>(dst[u]) = x[u];
+          *reinterpret_cast<Elements<T, kVec>*>(dst[u] + half) = y[u];
+        }
+      }
     }
   }
   // channels behind the last axis
@@ -149,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     int h = row - tt * heads;
     const int w = h >= a.heads[0];
     if (w) h -= a.heads[0];
-    static_cast<T*>(a.out[w])[out_at[w][tt] + (int64_t)h * a.D + ch] =
+    static_cast<T*>(a.out[w])[out_at[w][tt] + h * a.D + ch] =
         static_cast<const T*>(a.in[w])[in_at[w][tt] + h * a.stride[w][a.ndim + 1] + ch];
   }
 }
@@ -159,10 +178,10 @@ int launch(const RotaryArgs& a, int vec, int sms, cudaStream_t stream) {
   const int pairs = a.first_pair[a.axes];
   // As many tokens to a block as leave every SM four blocks; 16 at most.
   int64_t per = a.tokens / ((int64_t)sms * 4);
-  int block_tokens = (int)(per < 1 ? 1 : per > 16 ? 16 : per);
+  const int block_tokens = (int)(per < 1 ? 1 : per > kMostTokens ? kMostTokens : per);
   const int64_t blocks = (a.tokens + block_tokens - 1) / block_tokens;
   if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
-  const size_t smem = (size_t)block_tokens * pairs * sizeof(float2);
+  const size_t smem = (size_t)block_tokens * 2 * ((pairs + 3) / 4 * 4) * sizeof(float);
   switch (vec) {
     case 8: rotary_kernel<T, 8, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
     case 4: rotary_kernel<T, 4, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
@@ -223,6 +242,7 @@ extern "C" B200NA_API int b200na_rotary(
     a.origin[d] = origin ? (double)origin[d] : 0.0;
   }
   if (a.tokens == 0) return B200NA_OK;
+  a.batch_tokens = a.tokens / B;
   if (!query || !query_out || (Hkv > 0 && (!key || !key_out))) return B200NA_ERR_INVALID_ARGUMENT;
   a.in[0] = query;
   a.in[1] = key;
