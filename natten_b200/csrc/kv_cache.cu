@@ -11,170 +11,195 @@ namespace b200na {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;         // rows of keys and of values that a thread has in flight
+constexpr int kRows = 2;         // rows of keys and of values that a thread has in flight
 
 struct MoveArgs {
   PagedPool pool[2];             // keys, values
+  bool same_strides;             // of the two
   PageTable table;
-  void* data[2];                 // [B, T, heads, D]: given to the write, filled by the read
+  void* data[2];                 // [B, T, heads, D]: given to the write, filled (contiguous) by the read
   int64_t batch[2], token[2], head[2];   // its strides (elements)
   const int* start;
   const int* counts;
   int B, T, heads, D;
+  uint32_t heads_magic;          // ceil(2^32 / heads): x / heads = x * magic >> 32 for x * heads < 2^32
   int tokens;                    // of a block
   int tiles;                     // blocks of a sequence
 };
+
+// The largest magnitude of a piece as bits: magnitudes of floats are ordered like their bits, infinities and
+// NaNs come after all finite ones. 16-bit types: two maxima side by side.
+template <class T, int kVec> __device__ __forceinline__ uint32_t largest_bits(const Raw<T, kVec>& x, uint32_t most) {
+  if constexpr (sizeof(T) * kVec == 2) {
+    return __vmaxu2(most, (uint32_t)x & 0x7fffu);
+  } else {
+    uint32_t w[sizeof(T) * kVec / 4];
+    memcpy(w, &x, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * kVec / 4); ++i)
+      most = sizeof(T) == 2 ? __vmaxu2(most, w[i] & 0x7fff7fffu) : max(most, w[i] & 0x7fffffffu);
+    return most;
+  }
+}
 
 // Lanes per row: a power of two that holds D / kVec accesses, 32 at most (then several each).
 template <class T, class P, int kVec, bool kWrite>
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes_log2) {
   constexpr int kMost = kVec >= 8 ? 1 : kVec >= 4 ? 2 : 8;    // accesses a lane makes of one row, D <= 256
-  constexpr int kAtOnce = kMost == 8 ? 1 : kRows / (kMost * (int)sizeof(T) * kVec > 16 ? 2 : 1);
+  constexpr int kAtOnce = kMost == 8 ? 1 : kRows;
   constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  using In = Raw<T, kVec>;
+  using Cached = Raw<P, kVec>;
+  const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
   const int group = threadIdx.x >> lanes_log2, groups = kThreads >> lanes_log2;
   const int b = blockIdx.x / a.tiles, t0 = (blockIdx.x - b * a.tiles) * a.tokens;
   const int count = a.counts ? min(a.counts[b], a.T) : a.T;          // tokens that are moved
   const int here = min(a.tokens, (kWrite ? count : a.T) - t0);       // rows of tokens t0 + [0, here)
   if (here <= 0) return;
   const int64_t start = a.start ? a.start[b] : 0;
+  const int* const entries = a.table.entry + b * a.table.stride;
   const int accesses = a.D / kVec, rows = here * a.heads;
+  const bool my[2] = {lane < accesses, lane + (1 << lanes_log2) < accesses};
+  const auto mine = [&](int i) { return i < 2 ? my[i] : lane + (i << lanes_log2) < accesses; };
+  // this lane's piece of the first row
+  T* data[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+    data[w] = static_cast<T*>(a.data[w]) + b * a.batch[w] + t0 * a.token[w] + lane * kVec;
+  const int step = kVec << lanes_log2;                               // elements between a lane's accesses
   // (every lane of a warp takes part in every round: the shuffles below need them all)
   for (int row0 = 0; row0 < rows; row0 += groups * kAtOnce) {
-    using In = Raw<T, kVec>;
-    using Cached = Raw<P, kVec>;
     In x[kAtOnce][2][kMost];
     bool live[kAtOnce];
-    int t[kAtOnce], h[kAtOnce];
-    int64_t page[kAtOnce];
-    int slot[kAtOnce];
+    int h[kAtOnce], slot[kAtOnce], page[kAtOnce];
+    T* at[kAtOnce][2];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       const int row = row0 + u * groups + group;
       live[u] = row < rows;
-      const int tt = live[u] ? (int)((uint32_t)row / (uint32_t)a.heads) : 0;
-      h[u] = live[u] ? row - tt * a.heads : 0;
-      t[u] = t0 + tt;
-    }
-    if (kWrite) {
+      const int tt = a.heads == 1 ? row : (int)__umulhi(row, a.heads_magic);
+      h[u] = row - tt * a.heads;
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
+      for (int w = 0; w < 2; ++w) {
+        at[u][w] = kWrite ? data[w] + tt * a.token[w] + h[u] * a.head[w] : data[w] + (int64_t)row * a.D;
+        if (kWrite) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const T* data = static_cast<const T*>(a.data[w]) + b * a.batch[w] + t[u] * a.token[w] + h[u] * a.head[w];
-#pragma unroll
-          for (int i = 0; i < kMost; ++i)
-            if (live[u] && lane + (i << lanes_log2) < accesses)
-              x[u][w][i] = *reinterpret_cast<const In*>(data + (lane + (i << lanes_log2)) * kVec);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      page[u] = -1;
-      slot[u] = 0;
-      const int64_t p = start + t[u];
-      if (live[u] && t[u] < count && p >= 0) {
-        int64_t index;
-        a.table.split(p, &index, &slot[u]);
-        page[u] = a.table.page_of(b, index);
-      }
-    }
-    if (kWrite) {
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const bool to = page[u] >= 0;
-        float inverse[2] = {1.f, 1.f};
-        if constexpr (kScaled) {
-          float most[2] = {0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int i = 0; i < kMost; ++i)
-              if (live[u] && lane + (i << lanes_log2) < accesses) {
-                float f[kVec];
-                to_floats<T, kVec>(x[u][w][i], f);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                  const float m = fabsf(f[e]);
-                  most[w] = fmaxf(most[w], m < INFINITY ? m : INFINITY);   // infinity also for a NaN
-                }
-              }
-          for (int o = lanes / 2; o > 0; o >>= 1)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) most[w] = fmaxf(most[w], __shfl_xor_sync(0xffffffffu, most[w], o));
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            // not finite: the whole row reads back as NaN
-            const float scale = most[w] < INFINITY ? fmaxf(__fdiv_rn(most[w], kE4m3Max), kSmallestScale)
-                                                   : __int_as_float(0x7fc00000);
-            inverse[w] = __frcp_rn(scale);
-            const PagedPool& pool = a.pool[w];
-            if (to && lane == 0)
-              pool.scale[page[u] * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head] = scale;
+          for (int i = 0; i < kMost; ++i) {
+            x[u][w][i] = In{};
+            if (live[u] && mine(i)) x[u][w][i] = *reinterpret_cast<const In*>(at[u][w] + i * step);
           }
         }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const PagedPool& pool = a.pool[w];
-          P* const cached = static_cast<P*>(pool.base) + (to ? page[u] * pool.page + slot[u] * pool.token + h[u] * pool.head : 0);
-#pragma unroll
-          for (int i = 0; i < kMost; ++i)
-            if (to && lane + (i << lanes_log2) < accesses) {
-              Cached y;
-              if constexpr (kScaled) {
-                float f[kVec];
-                to_floats<T, kVec>(x[u][w][i], f);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) f[e] *= inverse[w];
-                y = from_floats<P, kVec>(f);
-              } else {
-                y = x[u][w][i];
-              }
-              *reinterpret_cast<Cached*>(cached + (lane + (i << lanes_log2)) * kVec) = y;
-            }
-        }
       }
-    } else {
-      Cached y[kAtOnce][2][kMost];
-      float scale[kAtOnce][2];
+      page[u] = -1;
+      slot[u] = 0;
+      const int t = t0 + tt;
+      const int64_t p = start + t;
+      if (live[u] && t < count && p >= 0) {
+        uint32_t index = (uint32_t)p;                                // (start and t are 31 bits each)
+        if (a.table.shift >= 0) {
+          index >>= a.table.shift;
+          slot[u] = (uint32_t)p & (a.table.page_size - 1);
+        } else {
+          index /= (uint32_t)a.table.page_size;
+          slot[u] = (uint32_t)p - index * a.table.page_size;
+        }
+        if (index < (uint32_t)a.table.max_pages) page[u] = entries[index];
+        if ((uint32_t)page[u] >= (uint32_t)a.table.pages) page[u] = -1;
+      }
+    }
+    Cached y[kAtOnce][2][kMost];
+    float scale[kAtOnce][2];
+    int64_t scale_at[kAtOnce][2];
+    P* cached[kAtOnce][2];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int pg = page[u] >= 0 ? page[u] : 0;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const PagedPool& pool = a.pool[w];
-          const bool from = page[u] >= 0;
-          scale[u][w] = 0.f;
-          if (kScaled && from)
-            scale[u][w] = pool.scale[page[u] * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head];
-          const P* const cached = static_cast<const P*>(pool.base) + (from ? page[u] * pool.page + slot[u] * pool.token + h[u] * pool.head : 0);
+      for (int w = 0; w < 2; ++w) {
+        const PagedPool& pool = a.pool[w];
+        const int64_t off = pg * pool.page + slot[u] * pool.token + h[u] * pool.head;
+        cached[u][w] = static_cast<P*>(pool.base) + (w && a.same_strides ? cached[u][0] - static_cast<P*>(a.pool[0].base) : off + lane * kVec);
+        if (kScaled) scale_at[u][w] = pg * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head;
+        if (!kWrite) {
+          scale[u][w] = kScaled && page[u] >= 0 ? pool.scale[scale_at[u][w]] : 0.f;
 #pragma unroll
           for (int i = 0; i < kMost; ++i) {
             y[u][w][i] = Cached{};
-            if (from && lane + (i << lanes_log2) < accesses)
-              y[u][w][i] = *reinterpret_cast<const Cached*>(cached + (lane + (i << lanes_log2)) * kVec);
+            if (page[u] >= 0 && mine(i)) y[u][w][i] = *reinterpret_cast<const Cached*>(cached[u][w] + i * step);
           }
         }
+      }
+    }
+    if constexpr (kWrite && kScaled) {
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
+      for (int u = 0; u < kAtOnce; ++u) {
+        uint32_t most[2] = {0, 0};
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int i = 0; i < kMost; ++i) most[w] = largest_bits<T, kVec>(x[u][w][i], most[w]);
+        if constexpr (sizeof(T) == 2) {
+          // keys in the low half, values in the high one
+          uint32_t both = __vmaxu2(__byte_perm(most[0], most[1], 0x5410), __byte_perm(most[0], most[1], 0x7632));
+          for (int o = 1; o < 1 << lanes_log2; o <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+          scale[u][0] = as_float(bits_as<T>((uint16_t)both));
+          scale[u][1] = as_float(bits_as<T>((uint16_t)(both >> 16)));
+        } else {
+          for (int o = 1; o < 1 << lanes_log2; o <<= 1)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) most[w] = max(most[w], __shfl_xor_sync(0xffffffffu, most[w], o));
+          scale[u][0] = __int_as_float(most[0]);
+          scale[u][1] = __int_as_float(most[1]);
+        }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          T* const data = static_cast<T*>(a.data[w]) + b * a.batch[w] + t[u] * a.token[w] + h[u] * a.head[w];
+          // most / 448, correctly rounded (a product and Markstein's correction by its remainder); a row that
+          // is not finite reads back as NaN
+          const float m = scale[u][w], q = m * (1.f / kE4m3Max);
+          const float s = fmaxf(__fmaf_rn(__fmaf_rn(-kE4m3Max, q, m), 1.f / kE4m3Max, q), kSmallestScale);
+          scale[u][w] = m < INFINITY ? s : __int_as_float(0x7fc00000);
+          if (page[u] >= 0 && lane == 0) a.pool[w].scale[scale_at[u][w]] = scale[u][w];
+        }
+      }
+    }
 #pragma unroll
-          for (int i = 0; i < kMost; ++i)
-            if (live[u] && lane + (i << lanes_log2) < accesses) {
-              if constexpr (kScaled) {
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        float factor = 1.f;
+        if (kScaled) factor = kWrite ? __frcp_rn(scale[u][w]) : scale[u][w];
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+          if constexpr (kWrite) {
+            if (page[u] < 0 || !mine(i)) continue;
+            if constexpr (kScaled) {
+              float f[kVec];
+              to_floats<T, kVec>(x[u][w][i], f);
+#pragma unroll
+              for (int e = 0; e < kVec; ++e) f[e] *= factor;
+              y[u][w][i] = from_floats<P, kVec>(f);
+            } else {
+              y[u][w][i] = x[u][w][i];
+            }
+            *reinterpret_cast<Cached*>(cached[u][w] + i * step) = y[u][w][i];
+          } else {
+            if (!live[u] || !mine(i)) continue;
+            if constexpr (kScaled) {
+              x[u][w][i] = In{};
+              if (page[u] >= 0) {
                 float f[kVec];
                 to_floats<P, kVec>(y[u][w][i], f);
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) f[e] *= scale[u][w];
+                for (int e = 0; e < kVec; ++e) f[e] *= factor;
                 x[u][w][i] = from_floats<T, kVec>(f);
-              } else {
-                x[u][w][i] = y[u][w][i];
               }
-              *reinterpret_cast<In*>(data + (lane + (i << lanes_log2)) * kVec) = x[u][w][i];
+            } else {
+              x[u][w][i] = y[u][w][i];
             }
+            *reinterpret_cast<In*>(at[u][w] + i * step) = x[u][w][i];
+          }
         }
-    }
+      }
   }
 }
 
@@ -196,6 +221,9 @@ int launch(MoveArgs a, cudaStream_t stream) {
   const int rows = (kThreads >> lanes_log2) * kRows;
   a.tokens = rows > a.heads ? rows / a.heads : 1;
   a.tiles = (a.T + a.tokens - 1) / a.tokens;
+  a.heads_magic = a.heads == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / a.heads) + (((uint64_t)1 << 32) % a.heads != 0);
+  a.same_strides = a.pool[0].page == a.pool[1].page && a.pool[0].token == a.pool[1].token &&
+                   a.pool[0].head == a.pool[1].head;
   const int64_t blocks = (int64_t)a.B * a.tiles;
   if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   if (wide) move_kernel<T, P, kWide, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes_log2);

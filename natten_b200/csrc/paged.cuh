@@ -75,7 +75,7 @@ inline PageTable page_table(const b200na_kv_cache& c, const int* table, int64_t 
 
 inline int check_cache(const b200na_kv_cache* c, const int* table, int64_t table_stride, int max_pages,
                        int dtype, int B) {
-  if (!c || c->pages < 0 || c->pages > 0x7fffffff || c->page_size < 1 || c->heads < 1 || c->head_dim < 1 ||
+  if (!c || c->pages < 0 || c->pages > 0x7fffffff || c->page_size < 1 || c->heads < 1 || c->heads > 32768 || c->head_dim < 1 ||
       max_pages < 0 || B < 0 || (B > 1 && table_stride < 0))
     return B200NA_ERR_INVALID_ARGUMENT;
   if (c->head_dim > 256) return B200NA_ERR_UNSUPPORTED;

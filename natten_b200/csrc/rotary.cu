@@ -5,8 +5,8 @@
 //
 // Angles: a far position times a frequency needs more than 24 bits before it is reduced to one turn, so
 // position * (f / 2 pi) is formed and reduced in fp64 and only the fraction of a turn goes to the fp32
-// sincospi. A block works the angles of its tokens out once, into shared memory, and uses them for all
-// heads of queries and keys. The rest is a stream: every element is read once and written once.
+// sincospi. A block works the angles of its tokens out once, into shared memory, and its threads keep their
+// columns' cosines and sines while they go through the heads of queries and keys. The rest is a stream: every element is read once and written once.
 #include <cmath>
 
 #include "paged.cuh"
@@ -17,7 +17,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;   // head_dim <= 256
 constexpr int kMostTokens = 16;  // of a block
-constexpr int kUnroll = 2;
+constexpr int kUnroll = 4;
 
 struct RotaryArgs {
   const void* in[2];
@@ -87,80 +87,76 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
   __syncthreads();
 
-  const int heads = a.heads[0] + a.heads[1], rows = count * heads;
-  const int chunks = pairs / kVec, at_once = chunks > 0 ? kThreads / chunks : 0;
-  const int group = chunks > 0 ? threadIdx.x / chunks : 0;
-  if (group < at_once) {
-    const int pair = (threadIdx.x - group * chunks) * kVec;
+  // A thread keeps its token and its column: the cosines and sines stay in registers while it goes through
+  // the heads, kUnroll of them at a time so that their loads are under way together.
+  const int chunks = pairs / kVec;
+  const int slot = chunks > 0 ? threadIdx.x / chunks : 0;
+  const int per_token = chunks > 0 ? max(1, kThreads / chunks / block_tokens) : 0;   // threads of a column
+  const int tt = chunks > 0 ? slot % block_tokens : 0, first = slot / block_tokens;
+  if (tt < count && first < per_token) {
+    const int pair = (threadIdx.x - slot * chunks) * kVec;
     const int axis = (pair >= a.first_pair[1] && a.axes > 1) + (pair >= a.first_pair[2] && a.axes > 2);
     const int half = kInterleaved ? 1 : a.first_pair[axis + 1] - a.first_pair[axis];
     const int lo = kInterleaved ? 2 * pair : a.first_pair[axis] + pair;     // 2 first + (pair - first)
-    const int64_t head_stride[2] = {a.stride[0][a.ndim + 1], a.stride[1][a.ndim + 1]};
-    int tt = group / heads, h = group - tt * heads;
-    for (int row = group; row < rows; row += kUnroll * at_once) {
-      // kUnroll rows at a time: their loads are under way together
-      Elements<T, kVec> x[kUnroll], y[kUnroll];
-      T* dst[kUnroll];
-      const float* table[kUnroll];
+    alignas(16) float cosine[kVec], sine[kVec];
+    constexpr int kLoad = kVec < 4 ? kVec : 4;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        dst[u] = nullptr;
-        if (row + u * at_once < rows) {
-          const int w = h >= a.heads[0], hh = w ? h - a.heads[0] : h;
-          const T* const src = static_cast<const T*>(a.in[w]) + in_at[w][tt] + hh * head_stride[w] + lo;
-          dst[u] = static_cast<T*>(a.out[w]) + out_at[w][tt] + hh * a.D + lo;
-          table[u] = cs + 2 * tt * stride + pair;
-          if constexpr (kInterleaved && kVec > 1) {
-            const Elements<T, 2 * kVec> both = *reinterpret_cast<const Elements<T, 2 * kVec>*>(src);
+    for (int e = 0; e < kVec; e += kLoad) {
+      *reinterpret_cast<Elements<float, kLoad>*>(cosine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(cs + 2 * tt * stride + pair + e);
+      *reinterpret_cast<Elements<float, kLoad>*>(sine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(cs + (2 * tt + 1) * stride + pair + e);
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int64_t head_stride = a.stride[w][a.ndim + 1];
+      const T* src = static_cast<const T*>(a.in[w]) + in_at[w][tt] + first * head_stride + lo;
+      T* dst = static_cast<T*>(a.out[w]) + out_at[w][tt] + first * a.D + lo;
+      const int64_t in_step = per_token * head_stride;
+      const int out_step = per_token * a.D;
+      for (int h = first; h < a.heads[w]; h += kUnroll * per_token) {
+        constexpr int kWide = kInterleaved && kVec > 1 ? 2 * kVec : kVec;
+        using Piece = Raw<T, kWide>;
+        Piece x[kUnroll], y[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (h + u * per_token < a.heads[w]) {
+            x[u] = *reinterpret_cast<const Piece*>(src + u * in_step);
+            if (kWide == kVec) y[u] = *reinterpret_cast<const Piece*>(src + u * in_step + half);
+          }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (h + u * per_token >= a.heads[w]) continue;
+          T* const to = dst + u * out_step;
+          if constexpr (kWide == kVec) {
+            float p[kVec], q[kVec];
+            to_floats<T, kVec>(x[u], p);
+            to_floats<T, kVec>(y[u], q);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-              x[u].v[e] = both.v[2 * e];
-              y[u].v[e] = both.v[2 * e + 1];
+              const float v = p[e];
+              p[e] = v * cosine[e] - q[e] * sine[e];
+              q[e] = v * sine[e] + q[e] * cosine[e];
             }
+            *reinterpret_cast<Piece*>(to) = from_floats<T, kVec>(p);
+            *reinterpret_cast<Piece*>(to + half) = from_floats<T, kVec>(q);
           } else {
-            x[u] = *reinterpret_cast<const Elements<T, kVec>*>(src);
-            y[u] = *reinterpret_cast<const Elements<T, kVec>*>(src + half);
+            float p[kWide];
+            to_floats<T, kWide>(x[u], p);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+              const float v = p[2 * e], z = p[2 * e + 1];
+              p[2 * e] = v * cosine[e] - z * sine[e];
+              p[2 * e + 1] = v * sine[e] + z * cosine[e];
+            }
+            *reinterpret_cast<Piece*>(to) = from_floats<T, kWide>(p);
           }
         }
-        h += at_once;
-        while (h >= heads) {
-          h -= heads;
-          ++tt;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (!dst[u]) continue;
-        alignas(16) float cosine[kVec], sine[kVec];
-        constexpr int kLoad = kVec < 4 ? kVec : 4;
-#pragma unroll
-        for (int e = 0; e < kVec; e += kLoad) {
-          *reinterpret_cast<Elements<float, kLoad>*>(cosine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(table[u] + e);
-          *reinterpret_cast<Elements<float, kLoad>*>(sine + e) = *reinterpret_cast<const Elements<float, kLoad>*>(table[u] + stride + e);
-        }
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float c = cosine[e], s = sine[e];
-          const float p = as_float(x[u].v[e]), q = as_float(y[u].v[e]);
-          x[u].v[e] = from_float<T>(p * c - q * s);
-          y[u].v[e] = from_float<T>(p * s + q * c);
-        }
-        if constexpr (kInterleaved && kVec > 1) {
-          Elements<T, 2 * kVec> both;
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            both.v[2 * e] = x[u].v[e];
-            both.v[2 * e + 1] = y[u].v[e];
-          }
-          *reinterpret_cast<Elements<T, 2 * kVec>*>(dst[u]) = both;
-        } else {
-          *reinterpret_cast<Elements<T, kVec>*>(dst[u]) = x[u];
-          *reinterpret_cast<Elements<T, kVec>*>(dst[u] + half) = y[u];
-        }
+        src += kUnroll * in_step;
+        dst += kUnroll * out_step;
       }
     }
   }
   // channels behind the last axis
+  const int heads = a.heads[0] + a.heads[1], rows = count * heads;
   const int turned = 2 * pairs, rest = a.D - turned;
   for (int i = threadIdx.x; i < rows * rest; i += kThreads) {
     const int row = i / rest, ch = turned + i - row * rest;
@@ -173,21 +169,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
 }
 
+template <class T, bool kInterleaved, int kVec>
+void launch_vec(const RotaryArgs& a, int vec, int block_tokens, unsigned blocks, size_t smem, cudaStream_t stream) {
+  if constexpr (kVec > 1) {
+    if (vec < kVec) return launch_vec<T, kInterleaved, kVec / 2>(a, vec, block_tokens, blocks, smem, stream);
+  }
+  rotary_kernel<T, kVec, kInterleaved><<<blocks, kThreads, smem, stream>>>(a, block_tokens);
+}
+
 template <class T, bool kInterleaved>
 int launch(const RotaryArgs& a, int vec, int sms, cudaStream_t stream) {
   const int pairs = a.first_pair[a.axes];
-  // As many tokens to a block as leave every SM four blocks; 16 at most.
-  int64_t per = a.tokens / ((int64_t)sms * 4);
-  const int block_tokens = (int)(per < 1 ? 1 : per > kMostTokens ? kMostTokens : per);
+  // As many tokens to a block as leave every SM eight blocks, but no more than its threads hold rows; a power
+  // of two, so that a token's columns fill whole warps.
+  const int64_t per = a.tokens / ((int64_t)sms * 8);
+  const int most = pairs >= vec ? kThreads / (pairs / vec) : kMostTokens;
+  int block_tokens = 1;
+  while (block_tokens * 2 <= per && block_tokens * 2 <= most && block_tokens * 2 <= kMostTokens) block_tokens *= 2;
   const int64_t blocks = (a.tokens + block_tokens - 1) / block_tokens;
   if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   const size_t smem = (size_t)block_tokens * 2 * ((pairs + 3) / 4 * 4) * sizeof(float);
-  switch (vec) {
-    case 8: rotary_kernel<T, 8, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
-    case 4: rotary_kernel<T, 4, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
-    case 2: rotary_kernel<T, 2, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
-    default: rotary_kernel<T, 1, kInterleaved><<<(unsigned)blocks, kThreads, smem, stream>>>(a, block_tokens); break;
-  }
+  launch_vec<T, kInterleaved, 16 / (int)sizeof(T) / (kInterleaved ? 2 : 1)>(a, vec, block_tokens, (unsigned)blocks, smem, stream);
   B200NA_CUDA_TRY(cudaGetLastError());
   return B200NA_OK;
 }
