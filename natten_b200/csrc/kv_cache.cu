@@ -5,6 +5,8 @@
 // access, so the largest magnitude of a row (for its 8-bit scale) is a few shuffles away and the row is
 // not read again. A block works on consecutive tokens of one sequence, so that a sequence's start and
 // count are read once a block and places need 32-bit arithmetic only; a thread has kRows rows in flight.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace b200na {
@@ -217,9 +219,14 @@ int launch(MoveArgs a, cudaStream_t stream) {
   const int accesses = wide ? a.D / kWide : a.D;
   int lanes_log2 = 0;
   while (lanes_log2 < 5 && (1 << lanes_log2) < accesses) ++lanes_log2;
-  // tokens of a block: one round of its threads' rows, at least one token
-  const int rows = (kThreads >> lanes_log2) * kRows;
-  a.tokens = rows > a.heads ? rows / a.heads : 1;
+  // Tokens of a block: rounds of its threads' rows, at least one token. More rounds (8 at most) share the wait
+  // for the sequence's count and start, as long as every SM keeps eight blocks.
+  int sms = 0;
+  const int rc = sm_count_of_current_device(&sms);
+  if (rc != B200NA_OK) return rc;
+  const int64_t round = (kThreads >> lanes_log2) * kRows, all = (int64_t)a.B * a.T * a.heads / round;
+  const int64_t rows = round * std::max<int64_t>(1, std::min<int64_t>(8, all / (8 * sms)));
+  a.tokens = rows > a.heads ? (int)rows / a.heads : 1;
   a.tiles = (a.T + a.tokens - 1) / a.tokens;
   a.heads_magic = a.heads == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / a.heads) + (((uint64_t)1 << 32) % a.heads != 0);
   a.same_strides = a.pool[0].page == a.pool[1].page && a.pool[0].token == a.pool[1].token &&
