@@ -8,11 +8,14 @@
 // counts is that all SMs read all the time, whatever the sequences' lengths are.
 //
 // Work: an item is one sequence, one key/value head and up to 16 (CUDA cores: 8) rows, which are the heads
-// of the group times neighbouring query tokens. Its keys are cut into units of 64 or 128. The units of all items
-// in a row are cut into as many equal ranges as there are blocks; lengths are read on the device, so the
-// host waits for nothing and a captured launch follows them. A block keeps the running maximum and sum of
-// each row over its range of an item and either writes the result (it had the whole item) or leaves a part
-// (at most two per block: the end of one item and the beginning of another). The second launch joins parts.
+// of the group times neighbouring query tokens. Its keys are cut into units, a tile for each warp of a block.
+// Lengths are read on the device, so the host waits for nothing and a captured launch follows them.
+//  - Few units at most (a window, a short table): a cluster of 1, 2, 4 or 8 blocks has an item, and joins its
+//    parts through distributed shared memory. One launch and no scratch.
+//  - Otherwise the units of all items in a row are cut into as many equal ranges as there are blocks on the GPU,
+//    whatever the sequences' lengths are. A block keeps the running maximum and sum of each row over its range
+//    of an item and either writes the result (it had the whole item) or leaves a part in scratch (at most two
+//    per block: the end of one item and the beginning of another). A second launch joins the parts.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -22,12 +25,16 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMostParts = 2 * 148;   // blocks of the first launch: two per SM
+#ifndef V_CU
+#define V_CU 8
+#endif
+constexpr int kClusterUnits = V_CU;      // units of an item that a block of a cluster takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DecodeArgs {
   const void* query;
   int64_t q_batch, q_token, q_head;
-  bool q_words;                       // 16-bit queries: every pair of channels lies on 4 bytes
+  bool q_wide;                        // 16-bit queries: every eight channels lie on 16 bytes
   void* out;
   float* lse;
   PagedPool key, value;
@@ -42,7 +49,8 @@ struct DecodeArgs {
   int item_tokens, item_heads;        // query tokens and heads of an item: its rows
   int token_blocks, head_blocks;
   uint32_t items;                     // of one sequence
-  int parts;
+  int cluster;                        // blocks that share an item; 0: ranges over all items, and the join
+  int parts;                          // blocks of those ranges
   int step;                           // keys that the warps of a block take at once: a tile each
   int unit;                           // keys of a unit of work, a multiple of `step`
   int2* covered;                      // [B * items]: first block that worked on the item, how many
@@ -131,22 +139,50 @@ struct Range {
   uint32_t before;       // units of all sequences before it
 };
 __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
-  __shared__ uint32_t sums[kWarps];
+  Range r;
+  if (a.cluster) {
+    // the block's share of its cluster's item, counted like the ranges below from the sequence's first unit
+    const uint32_t id = blockIdx.x / a.cluster, rank = blockIdx.x - id * a.cluster;
+    r.b = id / a.items;
+    r.length = a.lengths[r.b];
+    r.before = 0;
+    const uint32_t units = units_of(a, r.length), first = (id - r.b * a.items) * units;
+    const Split split(units, a.cluster);
+    r.begin = first + split.begin(rank);
+    r.end = first + split.begin(rank + 1);
+    r.total = r.parts = 0;
+    return r;
+  }
+  __shared__ uint32_t sums[2][kWarps];
   __shared__ uint32_t found_before;
   __shared__ int found_b, found_length;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // the first kThreads sequences, whose units are looked at again below
-  const int length0 = (int)threadIdx.x < a.B ? a.lengths[threadIdx.x] : 0;
-  const uint32_t units0 = (int)threadIdx.x < a.B ? units_of(a, length0) * a.items : 0;
-  uint32_t total = units0;
-  for (int b = threadIdx.x + kThreads; b < a.B; b += kThreads) total += units_of(a, a.lengths[b]) * a.items;
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) sums[warp] = total;
-  __syncthreads();
-  Range r;
-  r.total = 0;
+  const auto scan = [&](uint32_t x) {         // inclusive, over the warp
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) r.total += sums[w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  // the first kThreads sequences, a thread each, and the sum of the others
+  int length = (int)threadIdx.x < a.B ? a.lengths[threadIdx.x] : 0;
+  uint32_t mine = (int)threadIdx.x < a.B ? units_of(a, length) * a.items : 0, incl = scan(mine), others = 0;
+  for (int b = threadIdx.x + kThreads; b < a.B; b += kThreads) others += units_of(a, a.lengths[b]) * a.items;
+  others = __reduce_add_sync(0xffffffffu, others);
+  if (lane == 31) {
+    sums[0][warp] = incl;
+    sums[1][warp] = others;
+  }
+  __syncthreads();
+  r.total = 0;
+  uint32_t before = 0, chunk = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[0][w];
+    chunk += sums[0][w];
+    r.total += sums[0][w] + sums[1][w];
+  }
   r.parts = (int)min(r.total, (uint32_t)a.parts);
   r.begin = r.end = 0;
   r.b = r.length = 0;
@@ -155,36 +191,29 @@ __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
   const Split split(r.total, r.parts);
   r.begin = split.begin(blockIdx.x);
   r.end = split.begin(blockIdx.x + 1);
-  uint32_t before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    __syncthreads();
-    const int b = b0 + threadIdx.x;
-    const int length = b0 == 0 ? length0 : b < a.B ? a.lengths[b] : 0;
-    const uint32_t mine = b0 == 0 ? units0 : b < a.B ? units_of(a, length) * a.items : 0;
-    uint32_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    uint32_t base = before, chunk = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += sums[w];
-      chunk += sums[w];
-    }
-    const uint32_t lo = base + incl - mine;
+  for (int b0 = 0;;) {                        // the sequence with the range's first unit (always found)
+    const uint32_t lo = before + incl - mine;
     if (lo <= r.begin && r.begin < lo + mine) {
-      found_b = b;
+      found_b = b0 + threadIdx.x;
       found_length = length;
       found_before = lo;
     }
-    before += chunk;
-    if (r.begin < before) break;              // (the same for every thread)
+    __syncthreads();
+    b0 += kThreads;
+    if (r.begin < chunk || b0 >= a.B) break;  // (the same for every thread)
+    const int b = b0 + threadIdx.x;
+    length = b < a.B ? a.lengths[b] : 0;
+    mine = b < a.B ? units_of(a, length) * a.items : 0;
+    incl = scan(mine);
+    if (lane == 31) sums[0][warp] = incl;
+    __syncthreads();
+    before = chunk;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sums[0][w];
+      chunk += sums[0][w];
+    }
   }
-  __syncthreads();
   r.b = found_b;
   r.length = found_length;
   r.before = found_before;
@@ -192,10 +221,11 @@ __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
 }
 
 // How a segment (the block's part of an item) leaves: whole, or as part 0 (the item began in an earlier
-// block) or 1 of the block. The block that has the item's first unit notes which blocks the join has to
+// block) or 1 of the block; 2: as the block's part of its cluster's item. The block that has the item's first unit notes which blocks the join has to
 // look at.
 __device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, uint32_t item_begin,
                                        uint32_t item_end, int64_t item_id) {
+  if (a.cluster) return a.cluster == 1 ? -1 : 2;
   const bool begins = item_begin >= r.begin, ends = item_end <= r.end;
   if (begins && threadIdx.x == 0)
     a.covered[item_id] = make_int2(
@@ -203,12 +233,28 @@ __device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, uint
   return begins && ends ? -1 : begins ? 1 : 0;
 }
 
+// Final values of kN channels of a row.
+template <class T, int kN>
+__device__ __forceinline__ void write_row(const DecodeArgs& a, const Item& it, int row, int d, float m, float l,
+                                          const Elements<float, kN>& x) {
+  const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
+  const int64_t at = ((int64_t)it.b * a.T + t) * a.Hq + h;
+  Elements<T, kN> y;
+#pragma unroll
+  for (int e = 0; e < kN; ++e) y.v[e] = from_float<T>(m == -INFINITY ? 0.f : x.v[e] / l);
+  *reinterpret_cast<Elements<T, kN>*>(static_cast<T*>(a.out) + at * a.D + d) = y;
+  if (d == 0 && a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+// Where a block of a cluster keeps its part [rows_max][D]: behind its warps' outputs.
+__host__ __device__ __forceinline__ int joint_at(int o_stride, int rows_max) { return kWarps * rows_max * o_stride; }
+
 // Merges the warps' maxima, sums and outputs of the item's rows and writes them out. `o` holds the warps'
 // unnormalised outputs [kWarps][rows_max][o_stride], ml their (maximum, sum) [kWarps][rows_max]. kN channels
 // at a time.
 template <class T, int kN>
 __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int part, const float* o,
-                                      int o_stride, const float2* ml, int rows_max) {
+                                      int o_stride, const float2* ml, int rows_max,
+                                      float2* joint_ml) {
   const int rows = it.tokens * it.heads, pieces = a.D / kN;
   for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
     const int row = i / pieces, d = (i - row * pieces) * kN;
@@ -227,19 +273,71 @@ __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int p
       for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
     }
     if (part < 0) {
-      const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
-      const int64_t at = ((int64_t)it.b * a.T + t) * a.Hq + h;
-      Elements<T, kN> y;
-#pragma unroll
-      for (int e = 0; e < kN; ++e) y.v[e] = from_float<T>(m == -INFINITY ? 0.f : x.v[e] / l);
-      *reinterpret_cast<Elements<T, kN>*>(static_cast<T*>(a.out) + at * a.D + d) = y;
-      if (d == 0 && a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+      write_row<T, kN>(a, it, row, d, m, l, x);
+    } else if (part == 2) {
+      *reinterpret_cast<Elements<float, kN>*>(const_cast<float*>(o) + joint_at(o_stride, rows_max) + row * a.D + d) = x;
+      if (d == 0) joint_ml[row] = make_float2(m, l);
     } else {
       const int64_t slot = (int64_t)(2 * blockIdx.x + part) * rows_max + row;
       *reinterpret_cast<Elements<float, kN>*>(a.part_o + slot * a.D + d) = x;
       if (d == 0) a.part_ml[slot] = make_float2(m, l);
     }
   }
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same address in another block of the cluster.
+__device__ __forceinline__ uint32_t in_block(const void* p, uint32_t rank) {
+  uint32_t y;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  return y;
+}
+__device__ __forceinline__ float2 load_remote2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+  return v;
+}
+template <int kN> __device__ __forceinline__ Elements<float, kN> load_remote(uint32_t at) {
+  Elements<float, kN> v;
+  if constexpr (kN == 4)
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.v[0]), "=f"(v.v[1]), "=f"(v.v[2]), "=f"(v.v[3]) : "r"(at));
+  else
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v.v[0]) : "r"(at));
+  return v;
+}
+// The end of a cluster's item: every block has its part in shared memory; each joins a share of the channels.
+template <class T, int kN>
+__device__ __forceinline__ void join_cluster(const DecodeArgs& a, bool empty, const float* o, int o_stride,
+                                             float2* joint_ml, int rows_max) {
+  const uint32_t id = blockIdx.x / a.cluster, rank = blockIdx.x - id * a.cluster, b = id / a.items;
+  const Item it = rows_of(a, b, id - b * a.items);
+  const int rows = it.tokens * it.heads, pieces = a.D / kN;
+  if (empty)
+    for (int i = threadIdx.x; i < rows; i += kThreads) joint_ml[i] = make_float2(-INFINITY, 0.f);
+  cluster_barrier();
+  const float* const joint_o = o + joint_at(o_stride, rows_max);
+  for (int i = rank * kThreads + threadIdx.x; i < rows * pieces; i += a.cluster * kThreads) {
+    const int row = i / pieces, d = (i - row * pieces) * kN;
+    float m = -INFINITY, l = 0.f;
+    Elements<float, kN> x{};
+#pragma unroll 8
+    for (int z = 0; z < a.cluster; ++z) m = fmaxf(m, load_remote2(in_block(joint_ml + row, z)).x);
+#pragma unroll 8
+    for (int z = 0; z < a.cluster; ++z) {
+      const float2 p = load_remote2(in_block(joint_ml + row, z));
+      const Elements<float, kN> y = load_remote<kN>(in_block(joint_o + row * a.D + d, z));
+      if (p.x == -INFINITY) continue;         // (what `y` read was not written)
+      const float f = exp2f(p.x - m);
+      l += f * p.y;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
+    }
+    write_row<T, kN>(a, it, row, d, m, l, x);
+  }
+  cluster_barrier();                          // nobody leaves while others read
 }
 
 // ---- CUDA cores: fp32, and layouts that 16-byte copies cannot read -------------------------------------
@@ -252,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
   extern __shared__ float smem[];
   float* q = smem;                                      // [kRows][D]
   float* o = smem + kRows * a.D;                        // [kWarps][kRows][D]
-  __shared__ float2 ml[kWarps * kRows];
+  __shared__ float2 ml[kWarps * kRows], joint_ml[kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Range r = my_range(a);
   int b = r.b, length = r.length;
@@ -380,9 +478,10 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
-    leave<T, 1>(a, it, part, o, a.D, ml, kRows);
+    leave<T, 1>(a, it, part, o, a.D, ml, kRows, joint_ml);
     at = stop;
   }
+  if (a.cluster > 1) join_cluster<T, 1>(a, r.begin == r.end, o, a.D, joint_ml, kRows);
 }
 
 // ---- tensor cores: fp16 / bf16 queries, 16-byte rows ---------------------------------------------------
@@ -441,6 +540,11 @@ template <class M> __device__ __forceinline__ void mma(float (&c)[4], const uint
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // two e4m3 values (low 16 bits) -> two fp16 values
 __device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t x) {
   uint32_t y;
@@ -448,7 +552,7 @@ __device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t x) {
   return y;
 }
 
-template <int kDP, bool k8> struct Tile {
+template <int kDP, bool k8, int kRows> struct Tile {
   static constexpr int kRowBytes = kDP * (k8 ? 1 : 2);
   static constexpr int kChunks = kRowBytes / 16;                   // of a row
   static constexpr int kKeys = kRowBytes >= 256 ? 16 : 32;
@@ -456,11 +560,14 @@ template <int kDP, bool k8> struct Tile {
   static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
   static constexpr int kStage = 2 * kMatrix;
   static constexpr int kExtra = 16 + (k8 ? 2 * kKeys * 4 : 0);     // which keys are there; scales
-  static constexpr int kRows = 16;
+  static constexpr int kBlocks = kDP == 256 && !k8 ? 1 : 2;        // of an SM
+  static constexpr int kQueryPitch = kDP * 2 + 16;                 // bytes of a query row
+  // tiles, then what goes with them, then the queries; at an item's end results lie where the tiles were
+  static constexpr int kExtraAt = kWarps * kStages * kStage, kQueryAt = kExtraAt + kWarps * kStages * kExtra;
   static size_t bytes(int D) {
-    const size_t tiles = (size_t)kWarps * kStages * (kStage + kExtra);
-    const size_t merge = (size_t)kWarps * kRows * (D + 8) * sizeof(float);
-    return tiles > merge ? tiles : merge;
+    const size_t merge = ((size_t)joint_at(D + 8, kRows) + (size_t)kRows * D) * sizeof(float);
+    const size_t all = kQueryAt + 16 * kQueryPitch;
+    return all > merge ? all : merge;
   }
   // Byte of a chunk in a tile. Chunks of a row are permuted so that eight neighbouring rows have any one
   // chunk in eight different groups of banks; at(row, c ^ x) == at(row, c) ^ (x << 4).
@@ -481,24 +588,29 @@ template <class T, bool k8> __device__ __forceinline__ uint32_t not_finite(uint3
   return __vcmpeq2(x & e, e);
 }
 
-template <class T, bool k8, int kDP>
-__global__ void __launch_bounds__(kThreads, kDP == 256 && !k8 ? 1 : 2)
+// kRows 8: items of at most eight rows, so that the lower halves of the instructions' results are not looked at.
+template <class T, bool k8, int kDP, int kRows>
+__global__ void __launch_bounds__(kThreads, Tile<kDP, k8, kRows>::kBlocks)
 decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   using M = typename std::conditional<k8, __half, T>::type;        // operands of the products
-  using L = Tile<kDP, k8>;
+  using L = Tile<kDP, k8, kRows>;
   constexpr int kKeys = L::kKeys, kStages = L::kStages, kGroups = kKeys / 16, kSteps = kDP / 16;
+  constexpr int kX = kRows / 8, kE = 2 * kX;                       // rows and results of a fragment in use
+  // bf16 queries, 8-bit keys, eight rows: the products with the keys in 8 bits, see below
+  constexpr bool kSplit = k8 && kRows == 8 && std::is_same<T, __nv_bfloat16>::value;
   constexpr int kElem = k8 ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t tiles[];
-  __shared__ float2 ml[kWarps * 16];
+  __shared__ float2 ml[kWarps * kRows], joint_ml[kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = lane >> 2, c = lane & 3;                          // rows r0, r0 + 8 and columns 2c, 2c + 1
   uint8_t* const my_tiles = tiles + warp * kStages * L::kStage;
-  uint8_t* const my_extra = tiles + kWarps * kStages * L::kStage + warp * kStages * L::kExtra;
+  uint8_t* const my_extra = tiles + L::kExtraAt + warp * kStages * L::kExtra;
+  uint8_t* const queries = tiles + L::kQueryAt;
   const uint32_t tiles_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_tiles));
   const uint32_t extra_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_extra));
   // Copies: four lanes to a key, 64 bytes of its row at a time. Fragments: see the uses.
   const uint32_t copy_off = L::at(r0, c);
-  const uint32_t key_off = k8 ? L::at(lane & 15, lane >> 4) : L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
+  const uint32_t key_off = k8 && !kSplit ? L::at(lane & 15, lane >> 4) : L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
   const uint32_t value_off = L::kMatrix + L::at(lane & 15, lane >> 4);
   const int my_chunks = a.D * kElem / 16 - c;                      // chunks c, c + 4, .. that a row has
 
@@ -587,73 +699,105 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       look_up(s + 1);
     }
 
-    // The queries as A fragments: rows r0 and r0 + 8. 16-bit caches: channels 16 k + 2c, + 1 and 8 further;
-    // 8-bit ones: 16 k + 4c .. + 3, the four that one 32-bit word of a key row holds.
-    uint32_t q[kSteps][4];
-    float row_scale[2];
-    int row_token[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = r0 + 8 * x;
-      row_token[x] = row / it.heads;
-      const T* src = nullptr;
-      if (row < rows) {
-        const int t = it.t0 + row_token[x], h = it.head * a.group + it.h0 + row % it.heads;
-        src = static_cast<const T*>(a.query) + b * a.q_batch + t * a.q_token + h * a.q_head;
-      }
-      Elements<T, 2> v[kSteps][2];
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = 16 * k + (k8 ? 4 * c + 2 * e : 2 * c + 8 * e);
-          if (!src || d >= a.D) v[k][e].v[0] = v[k][e].v[1] = from_float<T>(0.f);
-          else if (a.q_words) v[k][e] = *reinterpret_cast<const Elements<T, 2>*>(src + d);
-          else {
-            v[k][e].v[0] = src[d];
-            v[k][e].v[1] = src[d + 1];
-          }
+    // The queries into shared memory, and from there as A fragments: rows r0 and r0 + 8.
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kRows * (kDP / 8); i += kThreads) {
+      const int row = i / (kDP / 8), d = i % (kDP / 8) * 8;
+      Raw<T, 8> piece{};
+      if (row < rows && d < a.D) {
+        const int tt = row / it.heads, h = it.head * a.group + it.h0 + row - tt * it.heads;
+        const T* const src = static_cast<const T*>(a.query) + b * a.q_batch + (it.t0 + tt) * a.q_token + h * a.q_head + d;
+        if (a.q_wide) {
+          piece = *reinterpret_cast<const Raw<T, 8>*>(src);
+        } else {
+          T x[8];
+          for (int e = 0; e < 8; ++e) x[e] = src[e];
+          memcpy(&piece, x, 16);
         }
+      }
+      *reinterpret_cast<Raw<T, 8>*>(queries + row * L::kQueryPitch + d * 2) = piece;
+    }
+    __syncthreads();
+    uint32_t q[kSplit ? kSteps / 2 : kSteps][4];
+    float row_scale[kX];
+    int row_token[kX];
+#pragma unroll
+    for (int x = 0; x < kX; ++x) {
+      row_token[x] = (r0 + 8 * x) / it.heads;
       row_scale[x] = a.scale_log2;
-      if constexpr (k8) {
-        float most = 0.f;
+    }
+    if constexpr (!k8) {
+      // channels 16 k + 2c, + 1 and 8 further
+      const uint32_t from = static_cast<uint32_t>(__cvta_generic_to_shared(queries)) +
+                            (kX == 2 ? lane & 15 : lane & 7) * L::kQueryPitch + (lane >> 4) * 16;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kSteps; ++k) {
+        ldmatrix4<false>(q[k], from + k * 32);
+        if (kX == 1) q[k][1] = q[k][3] = 0;
+      }
+    } else {
+      // channels 16 k + 4c .. + 3, the four that one 32-bit word of a key row holds
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            most = fmaxf(most, fmaxf(fabsf(as_float(v[k][e].v[0])), fabsf(as_float(v[k][e].v[1]))));
+      for (int x = 0; x < kX; ++x) {
+        float v[kSteps][4], most = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          to_floats<T, 4>(*reinterpret_cast<const Raw<T, 4>*>(queries + (r0 + 8 * x) * L::kQueryPitch + (16 * k + 4 * c) * 2), v[k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[k][e]));
+        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // 2^-e and 2^e of the largest magnitude's exponent, where both are normal numbers
-        const int e = (__float_as_int(most) >> 23) - 127;
+        // The row times the power of two that brings its largest magnitude to [1, 2) (kSplit: [128, 256)), where
+        // that power and its inverse are normal numbers.
+        constexpr int kUp = kSplit ? 7 : 0;
+        const int e = min((__float_as_int(most) >> 23) - 127, 126);
         float factor = 1.f;
-        if (e > -126 && e < 127) {
-          factor = __int_as_float((127 - e) << 23);
-          row_scale[x] *= __int_as_float((127 + e) << 23);
+        if (e > kUp - 126) {
+          factor = __int_as_float((127 + kUp - e) << 23);
+          row_scale[x] *= __int_as_float((127 - kUp + e) << 23);
         }
+        if constexpr (kSplit) {
+          if (!(most < INFINITY)) row_scale[x] = __int_as_float(0x7fc00000);    // e4m3 has no infinity
+          // A bf16 number is the sum of two e4m3 ones: the nearest one and what is left (four bits and sign,
+          // times 16). Row r0 of the instruction is the first, row r0 + 8 the second.
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+          for (int k = 0; k < kSteps; ++k) {
+            float left[4];
+            uint32_t hi = 0;
 #pragma unroll
-          for (int e2 = 0; e2 < 2; ++e2)
-            q[k][x + 2 * e2] = Half2Of<M>::pack(as_float(v[k][e2].v[0]) * factor, as_float(v[k][e2].v[1]) * factor);
-      } else {
+            for (int z = 0; z < 4; z += 2) {
+              const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[k][z] * factor, v[k][z + 1] * factor), __NV_SATFINITE, __NV_E4M3);
+              const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+              left[z] = 16.f * (v[k][z] * factor - back.x);
+              left[z + 1] = 16.f * (v[k][z + 1] * factor - back.y);
+              hi |= (uint32_t)two << (8 * z);
+            }
+            q[k / 2][2 * (k & 1)] = hi;
+            q[k / 2][2 * (k & 1) + 1] = from_floats<__nv_fp8_e4m3, 4>(left);
+          }
+        } else {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+          for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) q[k][x + 2 * e] = bits_as<uint32_t>(v[k][e]);
+            for (int z = 0; z < 2; ++z) {
+              q[k][x + 2 * z] = Half2Of<M>::pack(v[k][2 * z] * factor, v[k][2 * z + 1] * factor);
+              if (kX == 1) q[k][1 + 2 * z] = 0;
+            }
+        }
       }
     }
     // Tiles whose first key lies in [safe_from, safe_to] are attended whole, or not, by all rows alike.
     const bool alike = it.tokens == 1;
     const int64_t safe_from = (int64_t)it.p0 + it.tokens - a.window, safe_to = (int64_t)it.p0 - kKeys + 1;
 
-    float acc[kDP / 8][4], m[2], l[2], mv[2];
+    float acc[kDP / 8][4], m[kX], l[kX], mv[kX];
 #pragma unroll
     for (int i = 0; i < kDP / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < kX; ++x) {
       m[x] = mv[x] = -INFINITY;
       l[x] = 0.f;
     }
@@ -681,7 +825,19 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) part[z][i][e] = 0.f;
       const uint32_t keys = base + key_off;
-      if constexpr (!k8) {
+      if constexpr (kSplit) {
+        // 8-bit operands: the keys as they are, four times the rate of 16-bit ones (m16n8k32 4.5 cycles, the
+        // 16-bit m16n8k16 8 cycles) and no conversions. Both parts of the queries are exact, so are the products.
+#pragma unroll
+        for (int k = 0; k < kSteps / 2; ++k)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            uint32_t f[4];
+            ldmatrix4<false>(f, (keys ^ (k << 5)) + 16 * g * L::kRowBytes);
+            mma_e4m3(part[k % kChains][2 * g], q[k], f[0], f[1]);
+            mma_e4m3(part[k % kChains][2 * g + 1], q[k], f[2], f[3]);
+          }
+      } else if constexpr (!k8) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -705,13 +861,14 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
             }
           }
       }
-      float p[2 * kGroups][4], lv[2 * kGroups][2];
+      float p[2 * kGroups][kE], lv[2 * kGroups][2];
 #pragma unroll
       for (int i = 0; i < 2 * kGroups; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kE; ++e) {
           p[i][e] = part[0][i][e];
           if (kChains == 2) p[i][e] += part[kChains - 1][i][e];
+          if (kSplit) p[i][e] += 0.0625f * (kChains == 2 ? part[0][i][e + 2] + part[kChains - 1][i][e + 2] : part[0][i][e + 2]);
         }
         if constexpr (k8) {
           const float2 ks = *reinterpret_cast<const float2*>(extra + 16 + (8 * i + 2 * c) * 4);
@@ -719,7 +876,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           lv[i][0] = __log2f(vs.x);
           lv[i][1] = __log2f(vs.y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[i][e] *= e & 1 ? ks.y : ks.x;
+          for (int e = 0; e < kE; ++e) p[i][e] *= e & 1 ? ks.y : ks.x;
         }
       }
 
@@ -731,7 +888,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         uint32_t on[2] = {there, there};
         if (differ) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < kX; ++x) {
             const int upto = it.p0 + row_token[x] - j0 + 1;        // keys j <= p and j > p - window
             const int64_t from = upto - a.window;
             on[x] &= first_bits(upto) & ~first_bits(from > 0 ? (int)min(from, (int64_t)32) : 0);
@@ -740,14 +897,14 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
         for (int i = 0; i < 2 * kGroups; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < kE; ++e)
             if (!(on[e >> 1] >> (8 * i + 2 * c + (e & 1)) & 1)) p[i][e] = -INFINITY;
       }
 
       // the running maximum of the logits (and of the logits with the values' scales)
-      float base_m[2], base_v[2], keep[2];
+      float base_m[kX], base_v[kX], keep[kX];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < kX; ++x) {
         float top = -INFINITY, topv = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2 * kGroups; ++i)
@@ -774,18 +931,18 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           mv[x] = nextv;
         }
       }
-      if (__any_sync(0xffffffffu, !(keep[0] == 1.f && keep[1] == 1.f))) {
+      if (__any_sync(0xffffffffu, !(keep[0] == 1.f && keep[kX - 1] == 1.f))) {
 #pragma unroll
         for (int i = 0; i < kDP / 8; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][e] *= keep[e >> 1];
+          for (int e = 0; e < kE; ++e) acc[i][e] *= keep[e >> 1];
       }
       uint32_t w[kGroups][4];              // the weights as A fragments
 #pragma unroll
       for (int i = 0; i < 2 * kGroups; ++i) {
-        float y[4];
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kE; ++e) {
           const int x = e >> 1;
           const float ex = ex2(fmaf(p[i][e], row_scale[x], -base_m[x]));
           l[x] += ex;
@@ -811,7 +968,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
             uint32_t* const at_word = reinterpret_cast<uint32_t*>(values + L::at(key, i) + 4 * c);
             const uint32_t word = *at_word, odd = not_finite<T, k8>(word);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < kX; ++x) {
               const int back = upto + row_token[x];                         // p - j
               if (back < 0 || back >= a.window) continue;
 #pragma unroll
@@ -866,16 +1023,16 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     float* const o = reinterpret_cast<float*>(tiles);
     const int o_stride = a.D + 8;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < kX; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
       if (m[x] == -INFINITY && l[x] != l[x]) m[x] = 0.f;           // only NaN logits: they count
       const int row = r0 + 8 * x;
       if (row >= rows) continue;
-      if (c == 0) ml[warp * 16 + row] = make_float2(m[x], l[x]);
+      if (c == 0) ml[warp * kRows + row] = make_float2(m[x], l[x]);
       if (m[x] == -INFINITY) continue;                             // (not read)
       const float f = k8 ? ex2(mv[x] - m[x]) : 1.f;
-      float* const dst = o + (warp * 16 + row) * o_stride;
+      float* const dst = o + (warp * kRows + row) * o_stride;
       if constexpr (!k8) {
 #pragma unroll
         for (int i = 0; i < kDP / 8; ++i)
@@ -892,10 +1049,12 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
-    leave<T, 4>(a, it, part, o, o_stride, ml, 16);
-    __syncthreads();                                               // before the next item's tiles come
+    leave<T, 4>(a, it, part, o, o_stride, ml, kRows, joint_ml);
     at = stop;
+    if (at < r.end) __syncthreads();                               // before the next item's tiles come
   }
+  if (a.cluster > 1)
+    join_cluster<T, 4>(a, r.begin == r.end, reinterpret_cast<const float*>(tiles), a.D + 8, joint_ml, kRows);
 }
 
 // ---- the join --------------------------------------------------------------------------------------------
@@ -962,7 +1121,7 @@ struct Plan {
   bool tensor_cores;
   int rows_max;             // rows of an item
   int step, unit;
-  int item_tokens, item_heads, token_blocks, head_blocks, parts;
+  int item_tokens, item_heads, token_blocks, head_blocks, cluster, parts;
   int64_t items;
   int64_t covered_bytes, ml_bytes, o_bytes;
 };
@@ -989,13 +1148,14 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   const int group = Hq / cache->heads, D = cache->head_dim;
   p->tensor_cores = reads_in_chunks(*cache, dtype);
   p->rows_max = p->tensor_cores ? 16 : group == 1 && (T <= 1 || dilation > 1) ? 1 : 8;
-  // a tile for each of a block's warps
-  p->step = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
   p->item_heads = group < p->rows_max ? group : p->rows_max;
   p->head_blocks = (group + p->item_heads - 1) / p->item_heads;
   p->item_tokens = dilation > 1 ? 1 : p->rows_max / p->item_heads;
   if (p->item_tokens > T) p->item_tokens = T < 1 ? 1 : T;
+  if (p->item_tokens * p->item_heads <= 8 && p->rows_max > 8) p->rows_max = 8;
   p->token_blocks = (T + p->item_tokens - 1) / p->item_tokens;
+  // a tile for each of a block's warps
+  p->step = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
   p->items = (int64_t)cache->heads * p->token_blocks * p->head_blocks;
   if (B > 0 && p->items * p->rows_max > (int64_t)0x7fffffff / B) return B200NA_ERR_INVALID_ARGUMENT;
   // units if every sequence were as long as the table allows: larger ones where 31 bits would not count them
@@ -1007,6 +1167,15 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   const int64_t units = B * p->items * (most / p->unit + 1);
   if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   p->parts = (int)(units < kMostParts ? (units < 1 ? 1 : units) : kMostParts);
+  // Clusters, where a block of the largest that leave every block a place of its own has few units at most.
+  const int64_t item_units = most / p->unit + 1, item_count = B * p->items;
+  p->cluster = 1;
+  while (p->cluster < 8 && p->cluster * 2 <= item_units && item_count * p->cluster * 2 <= kMostParts) p->cluster *= 2;
+  if (item_units > kClusterUnits * p->cluster) p->cluster = 0;
+  if (p->cluster) {
+    p->covered_bytes = p->ml_bytes = p->o_bytes = 0;
+    return B200NA_OK;
+  }
   p->covered_bytes = round_up(B * p->items * (int64_t)sizeof(int2));
   p->ml_bytes = round_up((int64_t)2 * p->parts * p->rows_max * sizeof(float2));
   p->o_bytes = round_up((int64_t)2 * p->parts * p->rows_max * cache->head_dim * sizeof(float));
@@ -1015,19 +1184,34 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
 
 template <class K>
 int opt_in(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024)
+  if (bytes > 32 * 1024)   // (48 KB with the static arrays)
     B200NA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return B200NA_OK;
+}
+
+// The first launch: clusters that have an item each, or as many blocks as there are ranges.
+int launch(void (*kernel)(DecodeArgs), const DecodeArgs& a, size_t smem, cudaStream_t s) {
+  const int rc = opt_in(kernel, smem);
+  if (rc != B200NA_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.cluster ? (unsigned)a.B * a.items * a.cluster : (unsigned)a.parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  B200NA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   return B200NA_OK;
 }
 
 template <class T, class P, int kRows, int kD32, bool kWide>
 int launch_simt(const DecodeArgs& a, cudaStream_t s) {
-  const size_t smem = (size_t)(1 + kWarps) * kRows * a.D * sizeof(float);
-  const int rc = opt_in(decode_simt_kernel<T, P, kRows, kD32, kWide>, smem);
-  if (rc != B200NA_OK) return rc;
-  decode_simt_kernel<T, P, kRows, kD32, kWide><<<a.parts, kThreads, smem, s>>>(a);
-  B200NA_CUDA_TRY(cudaGetLastError());
-  return B200NA_OK;
+  const size_t smem = (size_t)(2 + kWarps) * kRows * a.D * sizeof(float);
+  return launch(decode_simt_kernel<T, P, kRows, kD32, kWide>, a, smem, s);
 }
 
 template <class T, class P>
@@ -1045,32 +1229,28 @@ int run_simt(const DecodeArgs& a, int rows_max, cudaStream_t s) {
   return a.D <= 128 ? launch_simt<T, P, 8, 4, false>(a, s) : launch_simt<T, P, 8, 8, false>(a, s);
 }
 
-template <class T, bool k8, int kDP>
+template <class T, bool k8, int kDP, int kRows>
 int launch_mma(const DecodeArgs& a, cudaStream_t s) {
-  const size_t smem = Tile<kDP, k8>::bytes(a.D);
-  const int rc = opt_in(decode_mma_kernel<T, k8, kDP>, smem);
-  if (rc != B200NA_OK) return rc;
-  decode_mma_kernel<T, k8, kDP><<<a.parts, kThreads, smem, s>>>(a);
-  B200NA_CUDA_TRY(cudaGetLastError());
-  return B200NA_OK;
+  return launch(decode_mma_kernel<T, k8, kDP, kRows>, a, Tile<kDP, k8, kRows>::bytes(a.D), s);
+}
+template <class T, bool k8, int kRows> int run_mma_rows(const DecodeArgs& a, cudaStream_t s) {
+  return a.D <= 64 ? launch_mma<T, k8, 64, kRows>(a, s)
+         : a.D <= 128 ? launch_mma<T, k8, 128, kRows>(a, s) : launch_mma<T, k8, 256, kRows>(a, s);
 }
 template <class T>
-int run_mma(const DecodeArgs& a, bool eight_bits, cudaStream_t s) {
+int run_mma(const DecodeArgs& a, bool eight_bits, int rows_max, cudaStream_t s) {
   if constexpr (!std::is_same<T, float>::value) {
-    if (eight_bits)
-      return a.D <= 64 ? launch_mma<T, true, 64>(a, s) : a.D <= 128 ? launch_mma<T, true, 128>(a, s)
-                                                                    : launch_mma<T, true, 256>(a, s);
-    return a.D <= 64 ? launch_mma<T, false, 64>(a, s) : a.D <= 128 ? launch_mma<T, false, 128>(a, s)
-                                                                   : launch_mma<T, false, 256>(a, s);
+    if (eight_bits) return rows_max == 8 ? run_mma_rows<T, true, 8>(a, s) : run_mma_rows<T, true, 16>(a, s);
+    return rows_max == 8 ? run_mma_rows<T, false, 8>(a, s) : run_mma_rows<T, false, 16>(a, s);
   }
   return B200NA_ERR_UNSUPPORTED;
 }
 
 template <class T>
 int run(const DecodeArgs& a, bool tensor_cores, int cache_dtype, int rows_max, cudaStream_t s) {
-  int rc = tensor_cores ? run_mma<T>(a, cache_dtype == B200NA_E4M3, s)
+  int rc = tensor_cores ? run_mma<T>(a, cache_dtype == B200NA_E4M3, rows_max, s)
            : cache_dtype == B200NA_E4M3 ? run_simt<T, __nv_fp8_e4m3>(a, rows_max, s) : run_simt<T, T>(a, rows_max, s);
-  if (rc != B200NA_OK) return rc;
+  if (rc != B200NA_OK || a.cluster) return rc;
   // The join's blocks may take their places while the first launch's last ones run (they wait for its end
   // before they read anything).
   cudaLaunchConfig_t cfg{};
@@ -1111,7 +1291,7 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   if (rc != B200NA_OK) return rc;
   if (!query_strides || !(scale > 0.f) || !(scale < INFINITY)) return B200NA_ERR_INVALID_ARGUMENT;
   if (B == 0 || T == 0) return B200NA_OK;
-  if (!query || !out || !lengths || !workspace) return B200NA_ERR_INVALID_ARGUMENT;
+  if (!query || !out || !lengths || (!workspace && !p.cluster)) return B200NA_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) % 16) return B200NA_ERR_ALIGNMENT;
   DecodeArgs a{};
   a.query = query;
@@ -1142,7 +1322,8 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.parts = p.parts;
   a.step = p.step;
   a.unit = p.unit;
-  a.q_words = reinterpret_cast<uintptr_t>(query) % 4 == 0 && (a.q_batch | a.q_token | a.q_head) % 2 == 0;
+  a.q_wide = reinterpret_cast<uintptr_t>(query) % 16 == 0 && (a.q_batch | a.q_token | a.q_head) % 8 == 0;
+  a.cluster = p.cluster;
   a.same_strides = a.key.page == a.value.page && a.key.token == a.value.token;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.covered = reinterpret_cast<int2*>(w);
