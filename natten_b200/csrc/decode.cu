@@ -25,16 +25,13 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMostParts = 2 * 148;   // blocks of the first launch: two per SM
-#ifndef V_CU
-#define V_CU 8
-#endif
-constexpr int kClusterUnits = V_CU;      // units of an item that a block of a cluster takes at most
+constexpr int kClusterUnits = 40;     // units of an item that a block of a cluster takes at most (see make_plan)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DecodeArgs {
   const void* query;
   int64_t q_batch, q_token, q_head;
-  bool q_wide;                        // 16-bit queries: every eight channels lie on 16 bytes
+  bool q_wide;                        // query rows lie on 16 bytes
   void* out;
   float* lse;
   PagedPool key, value;
@@ -340,13 +337,12 @@ __device__ __forceinline__ void join_cluster(const DecodeArgs& a, bool empty, co
   cluster_barrier();                          // nobody leaves while others read
 }
 
-// ---- CUDA cores: fp32, and layouts that 16-byte copies cannot read -------------------------------------
+// ---- CUDA cores: rows that 16-byte copies cannot read -------------------------------------------------------
 // A lane takes a key of a 32-key tile for the products with the queries, and every 32nd channel for the
 // products with the values.
-template <class T, class P, int kRows, int kD32, bool kWide>
+template <class T, class P, int kRows, int kD32>
 __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
   constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
-  constexpr int kVec = kWide ? 16 / (int)sizeof(P) : 1;
   extern __shared__ float smem[];
   float* q = smem;                                      // [kRows][D]
   float* o = smem + kRows * a.D;                        // [kWarps][kRows][D]
@@ -413,13 +409,11 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 #pragma unroll
       for (int x = 0; x < kRows; ++x) s[x] = 0.f;
       if (there)
-#pragma unroll 4
-        for (int d = 0; d < a.D; d += kVec) {
-          const Elements<P, kVec> kk = *reinterpret_cast<const Elements<P, kVec>*>(k + d);
+#pragma unroll 8
+        for (int d = 0; d < a.D; ++d) {
+          const float kk = as_float(k[d]);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e)
-#pragma unroll
-            for (int x = 0; x < kRows; ++x) s[x] += as_float(kk.v[e]) * q[x * a.D + d + e];
+          for (int x = 0; x < kRows; ++x) s[x] += kk * q[x * a.D + d];
         }
       uint32_t seen[kRows];
 #pragma unroll
@@ -552,28 +546,106 @@ __device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t x) {
   return y;
 }
 
-template <int kDP, bool k8, int kRows> struct Tile {
-  static constexpr int kRowBytes = kDP * (k8 ? 1 : 2);
+// Keys of a warp's tile: about 4 KB of them, for cached elements of `elem` bytes.
+__host__ __device__ constexpr int tile_keys(int row_bytes, int elem) {
+  return row_bytes >= 512 && elem == 4 ? 8 : row_bytes >= 256 ? 16 : 32;
+}
+
+// kElem: bytes of a cached element. k32: 32-bit queries (the CUDA-core kernel below).
+template <int kDP, int kElem, int kRows, bool k32> struct Tile {
+  static constexpr int kRowBytes = kDP * kElem;
   static constexpr int kChunks = kRowBytes / 16;                   // of a row
-  static constexpr int kKeys = kRowBytes >= 256 ? 16 : 32;
+  static constexpr int kKeys = tile_keys(kRowBytes, kElem);
   static constexpr int kStages = 3;
   static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
   static constexpr int kStage = 2 * kMatrix;
-  static constexpr int kExtra = 16 + (k8 ? 2 * kKeys * 4 : 0);     // which keys are there; scales
-  static constexpr int kBlocks = kDP == 256 && !k8 ? 1 : 2;        // of an SM
-  static constexpr int kQueryPitch = kDP * 2 + 16;                 // bytes of a query row
+  static constexpr int kExtra = 16 + (kElem == 1 ? 2 * kKeys * 4 : 0);     // which keys are there; scales
+  static constexpr int kBlocks = kDP == 256 && kElem > 1 ? 1 : 2;        // of an SM
+  static constexpr int kQueryPitch = k32 ? kDP * 4 : kDP * 2 + 16;   // bytes of a query row
   // tiles, then what goes with them, then the queries; at an item's end results lie where the tiles were
   static constexpr int kExtraAt = kWarps * kStages * kStage, kQueryAt = kExtraAt + kWarps * kStages * kExtra;
   static size_t bytes(int D) {
     const size_t merge = ((size_t)joint_at(D + 8, kRows) + (size_t)kRows * D) * sizeof(float);
-    const size_t all = kQueryAt + 16 * kQueryPitch;
+    const size_t all = kQueryAt + (k32 ? kRows : 16) * kQueryPitch;
     return all > merge ? all : merge;
   }
   // Byte of a chunk in a tile. Chunks of a row are permuted so that eight neighbouring rows have any one
   // chunk in eight different groups of banks; at(row, c ^ x) == at(row, c) ^ (x << 4).
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
-    const int x = kChunks >= 8 ? row & 7 : row >> 1 & 3;
+    // (32-bit queries: of two neighbouring rows, any four chunks c, c ^ 1, c ^ 2, c ^ 3)
+    const int x = kChunks < 8 ? row >> 1 & 3 : k32 ? (row & 1) << 2 | (row >> 1 & 3) : row & 7;
     return row * kRowBytes + ((chunk ^ x) << 4);
+  }
+};
+
+// What a warp does to get its tiles of an item's keys into shared memory.
+template <class L, bool k8, int kElem> struct Feed {
+  const DecodeArgs& a;
+  const Item& it;
+  const int* table;
+  const uint8_t *k_base, *v_base;
+  int begin, end, count;         // its first key, the end of the block's keys, its tiles
+  uint8_t* extra;                // the warp's, stage 0
+  uint32_t tiles_at, extra_at, copy_off;
+  int chunks;                    // c, c + 4, .. of a row, that there are
+  int page, slot;                // of this lane's key of the tile that is fetched next; page -1: there is none
+
+  // Looked up a tile before its copies are issued.
+  __device__ __forceinline__ void look_up(int s) {
+    const int i = begin + s * a.step + (threadIdx.x & 31 & (L::kKeys - 1));
+    page = -1;
+    slot = 0;
+    if (s < count && i < end) {
+      const uint32_t j = it.first + i * a.dilation;
+      uint32_t pi;
+      if (a.table.shift >= 0) {
+        pi = j >> a.table.shift;
+        slot = j & (a.table.page_size - 1);
+      } else {
+        pi = j / (uint32_t)a.table.page_size;
+        slot = j - pi * a.table.page_size;
+      }
+      if (pi < (uint32_t)a.table.max_pages) page = table[pi];
+      if ((uint32_t)page >= (uint32_t)a.table.pages) page = -1;
+    }
+  }
+  // Copies: four lanes to a key, 64 bytes of its row at a time.
+  __device__ __forceinline__ void fetch(int s, int stage) {
+    const int lane = threadIdx.x & 31, r0 = lane >> 2, c = lane & 3;
+    if (s < count) {
+      const bool there = page >= 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, there);
+      if (lane == 0) *reinterpret_cast<uint32_t*>(extra + stage * L::kExtra) = mask;
+      int64_t k_at = -1, v_at = -1;
+      if (there) {
+        k_at = (page * a.key.page + slot * a.key.token) * kElem;
+        v_at = a.same_strides ? k_at : (page * a.value.page + slot * a.value.token) * kElem;
+      }
+      const uint32_t dst = tiles_at + stage * L::kStage + copy_off;
+#pragma unroll
+      for (int g = 0; g < L::kKeys / 8; ++g) {
+        const int64_t ka = __shfl_sync(0xffffffffu, k_at, 8 * g + r0);
+        const int64_t va = a.same_strides ? ka : __shfl_sync(0xffffffffu, v_at, 8 * g + r0);
+        const uint8_t* const k = k_base + (ka >= 0 ? ka + c * 16 : 0);
+        const uint8_t* const v = v_base + (ka >= 0 ? va + c * 16 : 0);
+        const int n = ka >= 0 ? chunks : 0;                        // zeros where there is nothing
+#pragma unroll
+        for (int i = 0; i < L::kChunks / 4; ++i) {
+          const bool ok = 4 * i < n;
+          const uint32_t to = (dst ^ (i << 6)) + 8 * g * L::kRowBytes;
+          copy16(to, ok ? k + i * 64 : k_base, ok);
+          copy16(to + L::kMatrix, ok ? v + i * 64 : v_base, ok);
+        }
+      }
+      if (k8 && lane < L::kKeys) {
+        const int64_t ks = there ? page * a.key.s_page + slot * a.key.s_token + it.head * a.key.s_head : 0;
+        const int64_t vs = there ? page * a.value.s_page + slot * a.value.s_token + it.head * a.value.s_head : 0;
+        const uint32_t to = extra_at + stage * L::kExtra + 16 + lane * 4;
+        copy4(to, a.key.scale + ks, there);
+        copy4(to + L::kKeys * 4, a.value.scale + vs, there);
+      }
+    }
+    copy_commit();
   }
 };
 
@@ -590,10 +662,10 @@ template <class T, bool k8> __device__ __forceinline__ uint32_t not_finite(uint3
 
 // kRows 8: items of at most eight rows, so that the lower halves of the instructions' results are not looked at.
 template <class T, bool k8, int kDP, int kRows>
-__global__ void __launch_bounds__(kThreads, Tile<kDP, k8, kRows>::kBlocks)
+__global__ void __launch_bounds__(kThreads, Tile<kDP, k8 ? 1 : 2, kRows, false>::kBlocks)
 decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   using M = typename std::conditional<k8, __half, T>::type;        // operands of the products
-  using L = Tile<kDP, k8, kRows>;
+  using L = Tile<kDP, k8 ? 1 : 2, kRows, false>;
   constexpr int kKeys = L::kKeys, kStages = L::kStages, kGroups = kKeys / 16, kSteps = kDP / 16;
   constexpr int kX = kRows / 8, kE = 2 * kX;                       // rows and results of a fragment in use
   // bf16 queries, 8-bit keys, eight rows: the products with the keys in 8 bits, see below
@@ -608,7 +680,6 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   uint8_t* const queries = tiles + L::kQueryAt;
   const uint32_t tiles_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_tiles));
   const uint32_t extra_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_extra));
-  // Copies: four lanes to a key, 64 bytes of its row at a time. Fragments: see the uses.
   const uint32_t copy_off = L::at(r0, c);
   const uint32_t key_off = k8 && !kSplit ? L::at(lane & 15, lane >> 4) : L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
   const uint32_t value_off = L::kMatrix + L::at(lane & 15, lane >> 4);
@@ -631,72 +702,16 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     const int begin = (at - item_begin) * a.unit + warp * kKeys;
     const int end = (int)min((int64_t)(stop - item_begin) * a.unit, (int64_t)it.n);
     const int count = end > begin ? (end - begin + a.step - 1) / a.step : 0;          // this warp's tiles
-    const uint8_t* const k_base = static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem;
-    const uint8_t* const v_base = static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem;
-    const int* const table = a.table.entry + b * a.table.stride;
 
-    // Page and slot of this lane's key of tile `s`; page -1: there is none. Looked up a tile before its
-    // copies are issued.
-    int page, slot;
-    const auto look_up = [&](int s) {
-      const int i = begin + s * a.step + (lane & (kKeys - 1));
-      page = -1;
-      slot = 0;
-      if (s < count && i < end) {
-        const uint32_t j = it.first + i * a.dilation;
-        uint32_t pi;
-        if (a.table.shift >= 0) {
-          pi = j >> a.table.shift;
-          slot = j & (a.table.page_size - 1);
-        } else {
-          pi = j / (uint32_t)a.table.page_size;
-          slot = j - pi * a.table.page_size;
-        }
-        if (pi < (uint32_t)a.table.max_pages) page = table[pi];
-        if ((uint32_t)page >= (uint32_t)a.table.pages) page = -1;
-      }
-    };
-    const auto fetch = [&](int s, int stage) {
-      if (s < count) {
-        const bool there = page >= 0;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(my_extra + stage * L::kExtra) = mask;
-        int64_t k_at = -1, v_at = -1;
-        if (there) {
-          k_at = (page * a.key.page + slot * a.key.token) * kElem;
-          v_at = a.same_strides ? k_at : (page * a.value.page + slot * a.value.token) * kElem;
-        }
-        const uint32_t dst = tiles_at + stage * L::kStage + copy_off;
-#pragma unroll
-        for (int g = 0; g < kKeys / 8; ++g) {
-          const int64_t ka = __shfl_sync(0xffffffffu, k_at, 8 * g + r0);
-          const int64_t va = a.same_strides ? ka : __shfl_sync(0xffffffffu, v_at, 8 * g + r0);
-          const uint8_t* const k = k_base + (ka >= 0 ? ka + c * 16 : 0);
-          const uint8_t* const v = v_base + (ka >= 0 ? va + c * 16 : 0);
-          const int chunks = ka >= 0 ? my_chunks : 0;              // zeros where there is nothing
-#pragma unroll
-          for (int i = 0; i < L::kChunks / 4; ++i) {
-            const bool ok = 4 * i < chunks;
-            const uint32_t to = (dst ^ (i << 6)) + 8 * g * L::kRowBytes;
-            copy16(to, ok ? k + i * 64 : k_base, ok);
-            copy16(to + L::kMatrix, ok ? v + i * 64 : v_base, ok);
-          }
-        }
-        if (k8 && lane < kKeys) {
-          const int64_t ks = there ? page * a.key.s_page + slot * a.key.s_token + it.head * a.key.s_head : 0;
-          const int64_t vs = there ? page * a.value.s_page + slot * a.value.s_token + it.head * a.value.s_head : 0;
-          const uint32_t to = extra_at + stage * L::kExtra + 16 + lane * 4;
-          copy4(to, a.key.scale + ks, there);
-          copy4(to + kKeys * 4, a.value.scale + vs, there);
-        }
-      }
-      copy_commit();
-    };
-    look_up(0);
-#pragma unroll
+    Feed<L, k8, kElem> feed{a, it, a.table.entry + b * a.table.stride,
+                            static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem,
+                            static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem,
+                            begin, end, count, my_extra, tiles_at, extra_at, copy_off, my_chunks, -1, 0};
+    feed.look_up(0);
+#pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
-      fetch(s, s);
-      look_up(s + 1);
+      feed.fetch(s, s);
+      feed.look_up(s + 1);
     }
 
     // The queries into shared memory, and from there as A fragments: rows r0 and r0 + 8.
@@ -807,8 +822,8 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     for (int s = 0; s < count; ++s) {
       copy_wait<kStages - 2>();
       __syncwarp();                        // the tile is there, and everyone is done with the one before it
-      fetch(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
-      look_up(s + kStages);
+      feed.fetch(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+      feed.look_up(s + kStages);
       const uint32_t base = tiles_at + stage * L::kStage;
       const uint8_t* extra = my_extra + stage * L::kExtra;
       uint8_t* const values = my_tiles + stage * L::kStage + L::kMatrix;
@@ -1057,6 +1072,207 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     join_cluster<T, 4>(a, r.begin == r.end, reinterpret_cast<const float*>(tiles), a.D + 8, joint_ml, kRows);
 }
 
+// ---- CUDA cores: fp32 queries, 16-byte rows ----------------------------------------------------------------
+// fp32 products and sums. The same tiles and copies as above; eight keys at a time: four lanes to a key for the
+// products with the queries, every lane a share of the channels for the products with the values. A key costs
+// kRows x D multiply-adds for each of both against D cached elements of 4 bytes: at 8 rows 1/2 of what the
+// cores do while the memory delivers them.
+template <bool k8, int kDP, int kRows>
+__global__ void __launch_bounds__(kThreads, Tile<kDP, k8 ? 1 : 4, kRows, true>::kBlocks)
+decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
+  using L = Tile<kDP, k8 ? 1 : 4, kRows, true>;
+  using P = typename std::conditional<k8, __nv_fp8_e4m3, float>::type;
+  constexpr int kElem = k8 ? 1 : 4, kKeys = L::kKeys, kStages = L::kStages;
+  constexpr int kShare = L::kRowBytes / 32, kPiece = kShare < 16 ? kShare : 16;    // bytes of a value row for a lane
+  constexpr int kPieces = kShare / kPiece, kChannels = kPiece / kElem;             // pieces of them, channels each
+  constexpr int kOfChunk = 16 / kElem;                                             // channels of a chunk
+  extern __shared__ __align__(1024) uint8_t tiles[];
+  __shared__ float2 ml[kWarps * kRows], joint_ml[kRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = lane >> 2, c = lane & 3;
+  uint8_t* const my_tiles = tiles + warp * kStages * L::kStage;
+  uint8_t* const my_extra = tiles + L::kExtraAt + warp * kStages * L::kExtra;
+  float* const queries = reinterpret_cast<float*>(tiles + L::kQueryAt);            // [kRows][kDP]
+  const uint32_t tiles_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_tiles));
+  const uint32_t extra_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_extra));
+  const int my_chunks = a.D * kElem / 16 - c;
+
+  const Range r = my_range(a);
+  int b = r.b, length = r.length;
+  uint32_t before = r.before;
+  for (uint32_t at = r.begin; at < r.end;) {
+    const uint32_t units = units_of(a, length), index = (at - before) / units;
+    if (index >= a.items) {
+      before += units * a.items;
+      length = a.lengths[++b];
+      continue;
+    }
+    const Item it = item_of(a, b, index, length);
+    const uint32_t item_begin = before + index * units, item_end = item_begin + units;
+    const uint32_t stop = min(item_end, r.end);
+    const int rows = it.tokens * it.heads;
+    const int begin = (at - item_begin) * a.unit + warp * kKeys;
+    const int end = (int)min((int64_t)(stop - item_begin) * a.unit, (int64_t)it.n);
+    const int count = end > begin ? (end - begin + a.step - 1) / a.step : 0;          // this warp's tiles
+    Feed<L, k8, kElem> feed{a, it, a.table.entry + b * a.table.stride,
+                            static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem,
+                            static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem,
+                            begin, end, count, my_extra, tiles_at, extra_at, L::at(r0, c), my_chunks, -1, 0};
+    feed.look_up(0);
+#pragma unroll 1
+    for (int s = 0; s < kStages - 1; ++s) {
+      feed.fetch(s, s);
+      feed.look_up(s + 1);
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kRows * (kDP / 4); i += kThreads) {
+      const int row = i / (kDP / 4), d = i % (kDP / 4) * 4;
+      float4 piece = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows && d < a.D) {
+        const int tt = row / it.heads, h = it.head * a.group + it.h0 + row - tt * it.heads;
+        const float* const src = static_cast<const float*>(a.query) + b * a.q_batch + (it.t0 + tt) * a.q_token + h * a.q_head + d;
+        piece = a.q_wide ? *reinterpret_cast<const float4*>(src) : make_float4(src[0], src[1], src[2], src[3]);
+      }
+      *reinterpret_cast<float4*>(queries + row * kDP + d) = piece;
+    }
+    __syncthreads();
+    int row_token[kRows];
+    float acc[kRows][kPieces * kChannels], m[kRows], l[kRows];
+#pragma unroll
+    for (int x = 0; x < kRows; ++x) {
+      row_token[x] = x / it.heads;
+      m[x] = -INFINITY;
+      l[x] = 0.f;
+#pragma unroll
+      for (int e = 0; e < kPieces * kChannels; ++e) acc[x][e] = 0.f;
+    }
+    const int64_t safe_from = (int64_t)it.p0 + it.tokens - a.window, safe_to = (int64_t)it.p0 - kKeys + 1;
+
+    int stage = 0;
+#pragma unroll 1
+    for (int s = 0; s < count; ++s) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      feed.fetch(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+      feed.look_up(s + kStages);
+      const uint8_t* const keys = my_tiles + stage * L::kStage;
+      const uint8_t* const values = keys + L::kMatrix;
+      const uint8_t* const extra = my_extra + stage * L::kExtra;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      const uint32_t there = *reinterpret_cast<const uint32_t*>(extra) & first_bits(kKeys);
+      const int j0 = it.first + (begin + s * a.step) * a.dilation;
+      const bool differ = it.tokens > 1 && !(j0 >= safe_from && j0 <= safe_to);
+      const bool masked = there != first_bits(kKeys) || differ;
+      const auto attends = [&](int x, int key) {      // row x the key of the tile
+        const int back = it.p0 + row_token[x] - (j0 + key);
+        return (there >> key & 1) && (!differ || (back >= 0 && back < a.window));
+      };
+#pragma unroll 1
+      for (int key0 = 0; key0 < kKeys; key0 += 8) {
+        const int key = key0 + r0;
+        float p[kRows];
+#pragma unroll
+        for (int x = 0; x < kRows; ++x) p[x] = 0.f;
+#pragma unroll kRows == 8 ? (k8 ? 1 : 2) : 4
+        for (int i = 0; i < L::kChunks / 4; ++i) {
+          const int chunk = c + 4 * i;
+          float k[kOfChunk];
+          to_floats<P, kOfChunk>(*reinterpret_cast<const Raw<P, kOfChunk>*>(keys + L::at(key, chunk)), k);
+#pragma unroll
+          for (int x = 0; x < kRows; ++x)
+#pragma unroll
+            for (int e = 0; e < kOfChunk; e += 4) {
+              const float4 q = *reinterpret_cast<const float4*>(queries + x * kDP + chunk * kOfChunk + e);
+              p[x] = fmaf(q.x, k[e], p[x]);
+              p[x] = fmaf(q.y, k[e + 1], p[x]);
+              p[x] = fmaf(q.z, k[e + 2], p[x]);
+              p[x] = fmaf(q.w, k[e + 3], p[x]);
+            }
+        }
+        float factor = a.scale_log2, v_scale = 1.f;
+        if (k8) {
+          factor *= *reinterpret_cast<const float*>(extra + 16 + key * 4);
+          v_scale = *reinterpret_cast<const float*>(extra + 16 + (kKeys + key) * 4);
+        }
+        bool rescale = false;
+        float keep[kRows];
+#pragma unroll
+        for (int x = 0; x < kRows; ++x) {
+          p[x] += __shfl_xor_sync(0xffffffffu, p[x], 1);
+          p[x] += __shfl_xor_sync(0xffffffffu, p[x], 2);
+          const bool on = !masked || attends(x, key);
+          p[x] = on ? p[x] * factor : -INFINITY;
+          float top = p[x];
+#pragma unroll
+          for (int f = 4; f < 32; f <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, f));
+          const float next = fmaxf(m[x], top);
+          // nothing attended yet: no difference of infinities. (A NaN logit is passed over by the maximum and
+          // comes back in the exponential.)
+          const float base = next == -INFINITY ? 0.f : next;
+          keep[x] = exp2f(m[x] - base);
+          rescale = rescale || !(keep[x] == 1.f);
+          p[x] = exp2f(p[x] - base);
+          l[x] = l[x] * keep[x] + p[x];
+          m[x] = next;
+          if (k8) p[x] = on ? p[x] * v_scale : 0.f;
+        }
+        if (rescale) {                                 // (the same for every lane)
+#pragma unroll
+          for (int x = 0; x < kRows; ++x)
+#pragma unroll
+            for (int e = 0; e < kPieces * kChannels; ++e) acc[x][e] *= keep[x];
+        }
+#pragma unroll kRows == 8 ? 4 : 8
+        for (int z = 0; z < 8; ++z) {
+          float v[kPieces * kChannels];
+#pragma unroll
+          for (int y = 0; y < kPieces; ++y) {
+            const int off = (lane + 32 * y) * kPiece;
+            float part[kChannels];
+            to_floats<P, kChannels>(*reinterpret_cast<const Raw<P, kChannels>*>(values + L::at(key0 + z, off >> 4) + (off & 15)), part);
+#pragma unroll
+            for (int e = 0; e < kChannels; ++e) v[y * kChannels + e] = part[e];
+          }
+#pragma unroll
+          for (int x = 0; x < kRows; ++x) {
+            const float w = __shfl_sync(0xffffffffu, p[x], 4 * z);
+            // a NaN or an infinity stays with the rows that attend its token
+            if (masked && !attends(x, key0 + z)) continue;
+#pragma unroll
+            for (int e = 0; e < kPieces * kChannels; ++e) acc[x][e] = fmaf(w, v[e], acc[x][e]);
+          }
+        }
+      }
+    }
+
+    copy_wait<0>();
+    __syncthreads();
+    float* const o = reinterpret_cast<float*>(tiles);
+    const int o_stride = a.D + 8;
+#pragma unroll
+    for (int x = 0; x < kRows; ++x) {
+#pragma unroll
+      for (int f = 4; f < 32; f <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], f);
+      if (m[x] == -INFINITY && l[x] != l[x]) m[x] = 0.f;           // only NaN logits: they count
+      if (lane == 0) ml[warp * kRows + x] = make_float2(m[x], l[x]);
+#pragma unroll
+      for (int y = 0; y < kPieces; ++y)
+#pragma unroll
+        for (int e = 0; e < kChannels; ++e) {
+          const int d = (lane + 32 * y) * kChannels + e;
+          if (x < rows && d < a.D) o[(warp * kRows + x) * o_stride + d] = acc[x][y * kChannels + e];
+        }
+    }
+    __syncthreads();
+    const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
+    leave<float, 4>(a, it, part, o, o_stride, ml, kRows, joint_ml);
+    at = stop;
+    if (at < r.end) __syncthreads();                               // before the next item's tiles come
+  }
+  if (a.cluster > 1)
+    join_cluster<float, 4>(a, r.begin == r.end, reinterpret_cast<const float*>(tiles), a.D + 8, joint_ml, kRows);
+}
+
 // ---- the join --------------------------------------------------------------------------------------------
 // A warp per row of an item; items that one block had are done. A lane has a part's maximum and sum, then the
 // lanes share the channels.
@@ -1118,7 +1334,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
 // ---- host --------------------------------------------------------------------------------------------------
 
 struct Plan {
-  bool tensor_cores;
+  bool in_chunks;           // the kernels with tiles; otherwise rows that 16-byte copies cannot read
   int rows_max;             // rows of an item
   int step, unit;
   int item_tokens, item_heads, token_blocks, head_blocks, cluster, parts;
@@ -1126,11 +1342,10 @@ struct Plan {
   int64_t covered_bytes, ml_bytes, o_bytes;
 };
 
-// Whether the tensor-core kernel reads this cache: rows of whole 16-byte pieces on 16-byte boundaries, for
-// 16-bit queries.
-bool reads_in_chunks(const b200na_kv_cache& c, int dtype) {
-  if (dtype != B200NA_F16 && dtype != B200NA_BF16) return false;
-  const int per = c.dtype == B200NA_E4M3 ? 16 : 8;
+// Rows of whole 16-byte pieces on 16-byte boundaries.
+int elem_bytes(int dtype) { return dtype == B200NA_E4M3 ? 1 : dtype == B200NA_F32 ? 4 : 2; }
+bool reads_in_chunks(const b200na_kv_cache& c) {
+  const int per = 16 / elem_bytes(c.dtype);
   const PagedPool k = paged_pool(c, false), v = paged_pool(c, true);
   return c.head_dim % per == 0 &&
          (reinterpret_cast<uintptr_t>(c.key) | reinterpret_cast<uintptr_t>(c.value)) % 16 == 0 &&
@@ -1146,16 +1361,20 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   if (T < 0 || Hq < 1 || Hq % cache->heads || Hq > 65536 || kernel < 0 || dilation < 1)
     return B200NA_ERR_INVALID_ARGUMENT;
   const int group = Hq / cache->heads, D = cache->head_dim;
-  p->tensor_cores = reads_in_chunks(*cache, dtype);
-  p->rows_max = p->tensor_cores ? 16 : group == 1 && (T <= 1 || dilation > 1) ? 1 : 8;
+  p->in_chunks = reads_in_chunks(*cache);
+  const int single = group == 1 && (T <= 1 || dilation > 1);        // one row an item
+  p->rows_max = !p->in_chunks ? (single ? 1 : 8) : dtype == B200NA_F32 ? 8 : 16;
   p->item_heads = group < p->rows_max ? group : p->rows_max;
   p->head_blocks = (group + p->item_heads - 1) / p->item_heads;
   p->item_tokens = dilation > 1 ? 1 : p->rows_max / p->item_heads;
   if (p->item_tokens > T) p->item_tokens = T < 1 ? 1 : T;
-  if (p->item_tokens * p->item_heads <= 8 && p->rows_max > 8) p->rows_max = 8;
+  const int rows = p->item_tokens * p->item_heads;
+  if (p->rows_max == 16 && rows <= 8) p->rows_max = 8;
+  else if (p->in_chunks && dtype == B200NA_F32 && rows <= 2) p->rows_max = 2;
   p->token_blocks = (T + p->item_tokens - 1) / p->item_tokens;
   // a tile for each of a block's warps
-  p->step = kWarps * (p->tensor_cores && (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (cache->dtype == B200NA_E4M3 ? 1 : 2) >= 256 ? 16 : 32);
+  const int elem = elem_bytes(cache->dtype);
+  p->step = kWarps * (p->in_chunks ? tile_keys((D <= 64 ? 64 : D <= 128 ? 128 : 256) * elem, elem) : 32);
   p->items = (int64_t)cache->heads * p->token_blocks * p->head_blocks;
   if (B > 0 && p->items * p->rows_max > (int64_t)0x7fffffff / B) return B200NA_ERR_INVALID_ARGUMENT;
   // units if every sequence were as long as the table allows: larger ones where 31 bits would not count them
@@ -1167,10 +1386,13 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   const int64_t units = B * p->items * (most / p->unit + 1);
   if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   p->parts = (int)(units < kMostParts ? (units < 1 ? 1 : units) : kMostParts);
-  // Clusters, where a block of the largest that leave every block a place of its own has few units at most.
+  // Clusters of the largest size that leaves every block a place of its own, where a block's share is bounded.
+  // Against ranges and their join (us): 64 sequences, 4 heads, window 2048 (33 units) 49.5 / 57.6, window 512
+  // (9) 18.9 / 29.0; 1 sequence, window 2048 (33 over 8 blocks) 12.5 / 26.8; 4 sequences of 1000 to 8190 tokens (128
+  // over 8) 23.0 / 33.3. Beyond, ranges are right: lengths may differ by more than what the join costs.
   const int64_t item_units = most / p->unit + 1, item_count = B * p->items;
   p->cluster = 1;
-  while (p->cluster < 8 && p->cluster * 2 <= item_units && item_count * p->cluster * 2 <= kMostParts) p->cluster *= 2;
+  while (p->cluster < 8 && p->cluster < item_units && item_count * p->cluster * 2 <= kMostParts) p->cluster *= 2;
   if (item_units > kClusterUnits * p->cluster) p->cluster = 0;
   if (p->cluster) {
     p->covered_bytes = p->ml_bytes = p->o_bytes = 0;
@@ -1208,47 +1430,48 @@ int launch(void (*kernel)(DecodeArgs), const DecodeArgs& a, size_t smem, cudaStr
   return B200NA_OK;
 }
 
-template <class T, class P, int kRows, int kD32, bool kWide>
+template <class T, class P, int kRows, int kD32>
 int launch_simt(const DecodeArgs& a, cudaStream_t s) {
   const size_t smem = (size_t)(2 + kWarps) * kRows * a.D * sizeof(float);
-  return launch(decode_simt_kernel<T, P, kRows, kD32, kWide>, a, smem, s);
+  return launch(decode_simt_kernel<T, P, kRows, kD32>, a, smem, s);
 }
-
 template <class T, class P>
 int run_simt(const DecodeArgs& a, int rows_max, cudaStream_t s) {
-  constexpr int kVec = 16 / (int)sizeof(P);
-  if constexpr (std::is_same<T, float>::value) {
-    const bool wide = a.D % kVec == 0 && reinterpret_cast<uintptr_t>(a.key.base) % 16 == 0 &&
-                      (a.key.page | a.key.token | a.key.head) % kVec == 0;
-    if (wide) {
-      if (rows_max == 1) return a.D <= 128 ? launch_simt<T, P, 1, 4, true>(a, s) : launch_simt<T, P, 1, 8, true>(a, s);
-      return a.D <= 128 ? launch_simt<T, P, 8, 4, true>(a, s) : launch_simt<T, P, 8, 8, true>(a, s);
-    }
-  }
-  if (rows_max == 1) return a.D <= 128 ? launch_simt<T, P, 1, 4, false>(a, s) : launch_simt<T, P, 1, 8, false>(a, s);
-  return a.D <= 128 ? launch_simt<T, P, 8, 4, false>(a, s) : launch_simt<T, P, 8, 8, false>(a, s);
+  if (rows_max == 1) return a.D <= 128 ? launch_simt<T, P, 1, 4>(a, s) : launch_simt<T, P, 1, 8>(a, s);
+  return a.D <= 128 ? launch_simt<T, P, 8, 4>(a, s) : launch_simt<T, P, 8, 8>(a, s);
+}
+
+template <bool k8, int kDP, int kRows> int launch_fma(const DecodeArgs& a, cudaStream_t s) {
+  return launch(decode_fma_kernel<k8, kDP, kRows>, a, Tile<kDP, k8 ? 1 : 4, kRows, true>::bytes(a.D), s);
+}
+template <bool k8, int kRows> int run_fma(const DecodeArgs& a, cudaStream_t s) {
+  return a.D <= 64 ? launch_fma<k8, 64, kRows>(a, s)
+         : a.D <= 128 ? launch_fma<k8, 128, kRows>(a, s) : launch_fma<k8, 256, kRows>(a, s);
 }
 
 template <class T, bool k8, int kDP, int kRows>
 int launch_mma(const DecodeArgs& a, cudaStream_t s) {
-  return launch(decode_mma_kernel<T, k8, kDP, kRows>, a, Tile<kDP, k8, kRows>::bytes(a.D), s);
+  return launch(decode_mma_kernel<T, k8, kDP, kRows>, a, Tile<kDP, k8 ? 1 : 2, kRows, false>::bytes(a.D), s);
 }
 template <class T, bool k8, int kRows> int run_mma_rows(const DecodeArgs& a, cudaStream_t s) {
   return a.D <= 64 ? launch_mma<T, k8, 64, kRows>(a, s)
          : a.D <= 128 ? launch_mma<T, k8, 128, kRows>(a, s) : launch_mma<T, k8, 256, kRows>(a, s);
 }
+// rows of whole 16-byte pieces
 template <class T>
-int run_mma(const DecodeArgs& a, bool eight_bits, int rows_max, cudaStream_t s) {
-  if constexpr (!std::is_same<T, float>::value) {
+int run_tiles(const DecodeArgs& a, bool eight_bits, int rows_max, cudaStream_t s) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (eight_bits) return rows_max == 2 ? run_fma<true, 2>(a, s) : run_fma<true, 8>(a, s);
+    return rows_max == 2 ? run_fma<false, 2>(a, s) : run_fma<false, 8>(a, s);
+  } else {
     if (eight_bits) return rows_max == 8 ? run_mma_rows<T, true, 8>(a, s) : run_mma_rows<T, true, 16>(a, s);
     return rows_max == 8 ? run_mma_rows<T, false, 8>(a, s) : run_mma_rows<T, false, 16>(a, s);
   }
-  return B200NA_ERR_UNSUPPORTED;
 }
 
 template <class T>
-int run(const DecodeArgs& a, bool tensor_cores, int cache_dtype, int rows_max, cudaStream_t s) {
-  int rc = tensor_cores ? run_mma<T>(a, cache_dtype == B200NA_E4M3, rows_max, s)
+int run(const DecodeArgs& a, bool in_chunks, int cache_dtype, int rows_max, cudaStream_t s) {
+  int rc = in_chunks ? run_tiles<T>(a, cache_dtype == B200NA_E4M3, rows_max, s)
            : cache_dtype == B200NA_E4M3 ? run_simt<T, __nv_fp8_e4m3>(a, rows_max, s) : run_simt<T, T>(a, rows_max, s);
   if (rc != B200NA_OK || a.cluster) return rc;
   // The join's blocks may take their places while the first launch's last ones run (they wait for its end
@@ -1322,7 +1545,7 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.parts = p.parts;
   a.step = p.step;
   a.unit = p.unit;
-  a.q_wide = reinterpret_cast<uintptr_t>(query) % 16 == 0 && (a.q_batch | a.q_token | a.q_head) % 8 == 0;
+  a.q_wide = reinterpret_cast<uintptr_t>(query) % 16 == 0 && (a.q_batch | a.q_token | a.q_head) % (16 / elem_bytes(dtype)) == 0;
   a.cluster = p.cluster;
   a.same_strides = a.key.page == a.value.page && a.key.token == a.value.token;
   uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -1331,8 +1554,8 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.part_o = reinterpret_cast<float*>(w + p.covered_bytes + p.ml_bytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case B200NA_F32: return run<float>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
-    case B200NA_F16: return run<__half>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
-    default: return run<__nv_bfloat16>(a, p.tensor_cores, cache->dtype, p.rows_max, s);
+    case B200NA_F32: return run<float>(a, p.in_chunks, cache->dtype, p.rows_max, s);
+    case B200NA_F16: return run<__half>(a, p.in_chunks, cache->dtype, p.rows_max, s);
+    default: return run<__nv_bfloat16>(a, p.in_chunks, cache->dtype, p.rows_max, s);
   }
 }
