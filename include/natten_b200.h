@@ -496,8 +496,9 @@ B200NA_API int b200na_kv_cache_read(const b200na_kv_cache* cache, void* key, voi
  * query: [B, T, Hq, D] of `dtype` fp32 / fp16 / bf16, element strides of batch, token and head; Hq a
  * multiple of the cache's heads; the cache's dtype is the query's, or B200NA_E4M3. out: contiguous
  * [B, T, Hq, D], 16-byte aligned; lse: NULL or contiguous fp32 [B, T, Hq]. workspace:
- * b200na_na1d_decode_workspace(...) bytes, 16-byte aligned, for this call alone while it runs. Two
- * launches: parts of equal work whatever the lengths are, and their join.
+ * b200na_na1d_decode_workspace(...) bytes (0: none, NULL will do), 16-byte aligned, for this call alone
+ * while it runs. One launch where an item's keys are few at most (a window, a short table); otherwise
+ * two: parts of equal work whatever the lengths are, and their join. Tables of up to 2^31 - 4096 tokens.
  */
 B200NA_API int64_t b200na_na1d_decode_workspace(int B, int T, int Hq, const b200na_kv_cache* cache,
                                                 int max_pages, int kernel, int dilation, int dtype);

@@ -147,15 +147,18 @@ def test_decode_c_entry_refuses():
     assert _decode(_struct(), scale=0.0) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(), scale=float("inf")) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(), query=None) == L.ERR_INVALID_ARGUMENT
-    assert _decode(_struct(), workspace=None) == L.ERR_INVALID_ARGUMENT
+    # long tables work through ranges of all sequences' keys, which need scratch
+    assert _decode(_struct(), workspace=None, max_pages=10000) == L.ERR_INVALID_ARGUMENT
+    assert _decode(_struct(), max_pages=2 ** 28) == L.ERR_UNSUPPORTED        # 2^31 tokens
     assert _decode(_struct(), lengths=None) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(), table=None) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(), workspace=ctypes.c_void_p(1032)) == L.ERR_ALIGNMENT
     assert _decode(_struct(page_size=0)) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(key=None)) == L.ERR_INVALID_ARGUMENT
     assert _decode(_struct(), B=0) == L.OK and _decode(_struct(), T=0) == L.OK
-    size = L.lib.b200na_na1d_decode_workspace(2, 1, 2, ctypes.byref(_struct()), 3, 0, 1, L.BF16)
-    assert size > 0
+    sizes = [L.lib.b200na_na1d_decode_workspace(2, 1, 2, ctypes.byref(_struct()), pages, 0, 1, L.BF16)
+             for pages in (3, 10000)]
+    assert sizes[0] == 0 and sizes[1] > 0
     assert L.lib.b200na_na1d_decode_workspace(2, 1, 3, ctypes.byref(_struct()), 3, 0, 1,
                                               L.BF16) == L.ERR_INVALID_ARGUMENT
 
