@@ -46,10 +46,10 @@ struct DecodeArgs {
   int item_tokens, item_heads;        // query tokens and heads of an item: its rows
   int token_blocks, head_blocks;
   uint32_t items;                     // of one sequence
-  int cluster;                        // blocks that share an item; 0: ranges over all items, and the join
+  int cluster, cluster_log2;          // blocks that share an item; 0: ranges over all items, and the join
   int parts;                          // blocks of those ranges
   int step;                           // keys that the warps of a block take at once: a tile each
-  int unit;                           // keys of a unit of work, a multiple of `step`
+  int unit, unit_log2;                // keys of a unit of work, `step` times a power of two
   int2* covered;                      // [B * items]: first block that worked on the item, how many
   float2* part_ml;                    // [2 * parts][rows]: maximum (of scale_log2 * q.k) and sum
   float* part_o;                      // [2 * parts][rows][D]
@@ -63,14 +63,17 @@ __device__ __forceinline__ uint32_t units_of(const DecodeArgs& a, int length) {
   const int64_t widest = a.window + (a.dilation > 1 ? 0 : a.item_tokens - 1);
   n = n < a.capacity ? n : a.capacity;
   n = n < widest ? n : (int)widest;
-  return n > 0 ? ((uint32_t)n + a.unit - 1) / a.unit : 1;   // an item without keys still has its rows written
+  return n > 0 ? ((uint32_t)n + a.unit - 1) >> a.unit_log2 : 1;   // an item without keys still has its rows written
 }
 
 struct Item {
   int b, head, t0, tokens, h0, heads;
+  uint32_t heads_magic;  // row / heads = row * magic >> 16, for rows of an item
   int p0;                // position of token t0
   int first, n;          // keys at first + dilation * i, i < n
 };
+
+__device__ __forceinline__ int token_of(const Item& it, int row) { return row * it.heads_magic >> 16; }
 
 // The rows of an item: they do not depend on the sequence's length.
 __device__ __forceinline__ Item rows_of(const DecodeArgs& a, int b, uint32_t index) {
@@ -90,6 +93,7 @@ __device__ __forceinline__ Item rows_of(const DecodeArgs& a, int b, uint32_t ind
   it.tokens = min(a.item_tokens, a.T - it.t0);
   it.h0 = hb * a.item_heads;
   it.heads = min(a.item_heads, a.group - it.h0);
+  it.heads_magic = 65536u / it.heads + 1;
   return it;
 }
 
@@ -139,14 +143,13 @@ __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
   Range r;
   if (a.cluster) {
     // the block's share of its cluster's item, counted like the ranges below from the sequence's first unit
-    const uint32_t id = blockIdx.x / a.cluster, rank = blockIdx.x - id * a.cluster;
+    const uint32_t id = blockIdx.x >> a.cluster_log2, rank = blockIdx.x & (a.cluster - 1);
     r.b = id / a.items;
     r.length = a.lengths[r.b];
     r.before = 0;
     const uint32_t units = units_of(a, r.length), first = (id - r.b * a.items) * units;
-    const Split split(units, a.cluster);
-    r.begin = first + split.begin(rank);
-    r.end = first + split.begin(rank + 1);
+    r.begin = first + (units * rank >> a.cluster_log2);
+    r.end = first + (units * (rank + 1) >> a.cluster_log2);
     r.total = r.parts = 0;
     return r;
   }
@@ -234,8 +237,8 @@ __device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, uint
 template <class T, int kN>
 __device__ __forceinline__ void write_row(const DecodeArgs& a, const Item& it, int row, int d, float m, float l,
                                           const Elements<float, kN>& x) {
-  const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
-  const int64_t at = ((int64_t)it.b * a.T + t) * a.Hq + h;
+  const int tt = token_of(it, row), h = it.head * a.group + it.h0 + row - tt * it.heads;
+  const int64_t at = ((int64_t)it.b * a.T + it.t0 + tt) * a.Hq + h;
   Elements<T, kN> y;
 #pragma unroll
   for (int e = 0; e < kN; ++e) y.v[e] = from_float<T>(m == -INFINITY ? 0.f : x.v[e] / l);
@@ -252,32 +255,36 @@ template <class T, int kN>
 __device__ __forceinline__ void leave(const DecodeArgs& a, const Item& it, int part, const float* o,
                                       int o_stride, const float2* ml, int rows_max,
                                       float2* joint_ml) {
-  const int rows = it.tokens * it.heads, pieces = a.D / kN;
-  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
-    const int row = i / pieces, d = (i - row * pieces) * kN;
-    float m = -INFINITY, l = 0.f;
-    Elements<float, kN> x{};
+  const int rows = it.tokens * it.heads, lane = threadIdx.x & 31;
+  for (int row = threadIdx.x >> 5; row < rows; row += kWarps) {
+    float m = -INFINITY, l = 0.f, f[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * rows_max + row].x);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float2 p = ml[w * rows_max + row];
-      if (p.x == -INFINITY) continue;         // the warp met no key of this row
-      const float f = exp2f(p.x - m);
-      l += f * p.y;
-      const Elements<float, kN> y = *reinterpret_cast<const Elements<float, kN>*>(o + (w * rows_max + row) * o_stride + d);
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
+      f[w] = p.x == -INFINITY ? 0.f : exp2f(p.x - m);               // 0: the warp met no key of this row
+      l += p.x == -INFINITY ? 0.f : f[w] * p.y;
     }
-    if (part < 0) {
-      write_row<T, kN>(a, it, row, d, m, l, x);
-    } else if (part == 2) {
-      *reinterpret_cast<Elements<float, kN>*>(const_cast<float*>(o) + joint_at(o_stride, rows_max) + row * a.D + d) = x;
-      if (d == 0) joint_ml[row] = make_float2(m, l);
-    } else {
-      const int64_t slot = (int64_t)(2 * blockIdx.x + part) * rows_max + row;
-      *reinterpret_cast<Elements<float, kN>*>(a.part_o + slot * a.D + d) = x;
-      if (d == 0) a.part_ml[slot] = make_float2(m, l);
+    for (int d = lane * kN; d < a.D; d += 32 * kN) {
+      Elements<float, kN> x{};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (ml[w * rows_max + row].x == -INFINITY) continue;        // (what lies there was not written)
+        const Elements<float, kN> y = *reinterpret_cast<const Elements<float, kN>*>(o + (w * rows_max + row) * o_stride + d);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) x.v[e] += f[w] * y.v[e];
+      }
+      if (part < 0) {
+        write_row<T, kN>(a, it, row, d, m, l, x);
+      } else if (part == 2) {
+        *reinterpret_cast<Elements<float, kN>*>(const_cast<float*>(o) + joint_at(o_stride, rows_max) + row * a.D + d) = x;
+        if (d == 0) joint_ml[row] = make_float2(m, l);
+      } else {
+        const int64_t slot = (int64_t)(2 * blockIdx.x + part) * rows_max + row;
+        *reinterpret_cast<Elements<float, kN>*>(a.part_o + slot * a.D + d) = x;
+        if (d == 0) a.part_ml[slot] = make_float2(m, l);
+      }
     }
   }
 }
@@ -309,30 +316,39 @@ template <int kN> __device__ __forceinline__ Elements<float, kN> load_remote(uin
 template <class T, int kN>
 __device__ __forceinline__ void join_cluster(const DecodeArgs& a, bool empty, const float* o, int o_stride,
                                              float2* joint_ml, int rows_max) {
-  const uint32_t id = blockIdx.x / a.cluster, rank = blockIdx.x - id * a.cluster, b = id / a.items;
+  const uint32_t id = blockIdx.x >> a.cluster_log2, rank = blockIdx.x & (a.cluster - 1), b = id / a.items;
   const Item it = rows_of(a, b, id - b * a.items);
-  const int rows = it.tokens * it.heads, pieces = a.D / kN;
+  const int rows = it.tokens * it.heads, lane = threadIdx.x & 31;
   if (empty)
     for (int i = threadIdx.x; i < rows; i += kThreads) joint_ml[i] = make_float2(-INFINITY, 0.f);
   cluster_barrier();
   const float* const joint_o = o + joint_at(o_stride, rows_max);
-  for (int i = rank * kThreads + threadIdx.x; i < rows * pieces; i += a.cluster * kThreads) {
-    const int row = i / pieces, d = (i - row * pieces) * kN;
-    float m = -INFINITY, l = 0.f;
-    Elements<float, kN> x{};
-#pragma unroll 8
-    for (int z = 0; z < a.cluster; ++z) m = fmaxf(m, load_remote2(in_block(joint_ml + row, z)).x);
-#pragma unroll 8
-    for (int z = 0; z < a.cluster; ++z) {
-      const float2 p = load_remote2(in_block(joint_ml + row, z));
-      const Elements<float, kN> y = load_remote<kN>(in_block(joint_o + row * a.D + d, z));
-      if (p.x == -INFINITY) continue;         // (what `y` read was not written)
-      const float f = exp2f(p.x - m);
-      l += f * p.y;
+  for (int row = rank * kWarps + (threadIdx.x >> 5); row < rows; row += a.cluster * kWarps) {
+    // lane z has block z's maximum and sum
+    const float2 p = lane < a.cluster ? load_remote2(in_block(joint_ml + row, lane)) : make_float2(-INFINITY, 0.f);
+    float m = p.x;
 #pragma unroll
-      for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
+    for (int z = 4; z > 0; z >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, z));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    const float w = p.x == -INFINITY ? 0.f : exp2f(p.x - m);
+    float l = p.x == -INFINITY ? 0.f : w * p.y;
+#pragma unroll
+    for (int z = 4; z > 0; z >>= 1) l += __shfl_xor_sync(0xffffffffu, l, z);
+    l = __shfl_sync(0xffffffffu, l, 0);
+    const uint32_t there = __ballot_sync(0xffffffffu, p.x != -INFINITY);
+    for (int d0 = 0; d0 < a.D; d0 += 32 * kN) {
+      const int d = d0 + lane * kN;
+      Elements<float, kN> x{};
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        const float f = __shfl_sync(0xffffffffu, w, z);
+        if (!(there >> z & 1) || d >= a.D) continue;                // (what lies there was not written)
+        const Elements<float, kN> y = load_remote<kN>(in_block(joint_o + row * a.D + d, z));
+#pragma unroll
+        for (int e = 0; e < kN; ++e) x.v[e] += f * y.v[e];
+      }
+      if (d < a.D) write_row<T, kN>(a, it, row, d, m, l, x);
     }
-    write_row<T, kN>(a, it, row, d, m, l, x);
   }
   cluster_barrier();                          // nobody leaves while others read
 }
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
       const int row = i / a.D, d = i - row * a.D;
       float x = 0.f;
       if (row < rows) {
-        const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
+        const int tt = token_of(it, row), t = it.t0 + tt, h = it.head * a.group + it.h0 + row - tt * it.heads;
         x = as_float(static_cast<const T*>(a.query)[b * a.q_batch + t * a.q_token + h * a.q_head + d]);
       }
       q[i] = x;
@@ -418,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
       uint32_t seen[kRows];
 #pragma unroll
       for (int x = 0; x < kRows; ++x) {
-        const int p = it.p0 + (x < rows ? x / it.heads : 0);
+        const int p = it.p0 + token_of(it, x);
         const bool on = there && x < rows && (a.dilation > 1 || (j <= p && j > p - a.window));
         seen[x] = __ballot_sync(0xffffffffu, on);
         s[x] = on ? s[x] * k_scale * a.scale_log2 : -INFINITY;
@@ -506,8 +522,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
@@ -523,6 +539,12 @@ template <bool kTrans> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+// Two 16 x 16 matrices of bytes, transposed: register z of matrix y (2 y + z) has column lane / 4 + 8 z of rows
+// 4 (lane % 4) .. + 3.
+__device__ __forceinline__ void ldmatrix_bytes(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 template <class M> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (std::is_same<M, __half>::value)
@@ -576,6 +598,14 @@ template <int kDP, int kElem, int kRows, bool k32> struct Tile {
     const int x = kChunks < 8 ? row >> 1 & 3 : k32 ? (row & 1) << 2 | (row >> 1 & 3) : row & 7;
     return row * kRowBytes + ((chunk ^ x) << 4);
   }
+  // 8-bit keys for the tensor cores are read in rows 0, 1, 4, 5, 8, 9, 12, 13 and 2, 3, .. (see there).
+  static constexpr bool kPairs = kElem == 1 && !k32;
+  static constexpr uint32_t kOddGroup = kPairs ? (kChunks >= 8 ? 4 : 2) << 4 : 0;   // of the chunks of rows 8 .. 15
+  static __device__ __forceinline__ uint32_t key_at(int row, int chunk) {
+    if (!kPairs) return at(row, chunk);
+    const int x = kChunks >= 8 ? (row & 1) | (row >> 1 & 6) : row >> 2 & 3;
+    return row * kRowBytes + ((chunk ^ x) << 4);
+  }
 };
 
 // What a warp does to get its tiles of an item's keys into shared memory.
@@ -584,9 +614,10 @@ template <class L, bool k8, int kElem> struct Feed {
   const Item& it;
   const int* table;
   const uint8_t *k_base, *v_base;
+  const float *ks_base, *vs_base;
   int begin, end, count;         // its first key, the end of the block's keys, its tiles
   uint8_t* extra;                // the warp's, stage 0
-  uint32_t tiles_at, extra_at, copy_off;
+  uint32_t tiles_at, extra_at, key_off, value_off;   // (of the lane's copies)
   int chunks;                    // c, c + 4, .. of a row, that there are
   int page, slot;                // of this lane's key of the tile that is fetched next; page -1: there is none
 
@@ -618,31 +649,31 @@ template <class L, bool k8, int kElem> struct Feed {
       if (lane == 0) *reinterpret_cast<uint32_t*>(extra + stage * L::kExtra) = mask;
       int64_t k_at = -1, v_at = -1;
       if (there) {
-        k_at = (page * a.key.page + slot * a.key.token) * kElem;
-        v_at = a.same_strides ? k_at : (page * a.value.page + slot * a.value.token) * kElem;
+        k_at = a.key.at(page, slot) * kElem;
+        v_at = a.same_strides ? k_at : a.value.at(page, slot) * kElem;
       }
-      const uint32_t dst = tiles_at + stage * L::kStage + copy_off;
+      const uint32_t key_to = tiles_at + stage * L::kStage + key_off, value_to = tiles_at + stage * L::kStage + value_off;
 #pragma unroll
       for (int g = 0; g < L::kKeys / 8; ++g) {
         const int64_t ka = __shfl_sync(0xffffffffu, k_at, 8 * g + r0);
         const int64_t va = a.same_strides ? ka : __shfl_sync(0xffffffffu, v_at, 8 * g + r0);
+        // zeros where there is nothing: copies of no bytes, whose addresses are not looked at
         const uint8_t* const k = k_base + (ka >= 0 ? ka + c * 16 : 0);
         const uint8_t* const v = v_base + (ka >= 0 ? va + c * 16 : 0);
-        const int n = ka >= 0 ? chunks : 0;                        // zeros where there is nothing
+        const int n = ka >= 0 ? chunks : 0;
 #pragma unroll
         for (int i = 0; i < L::kChunks / 4; ++i) {
-          const bool ok = 4 * i < n;
-          const uint32_t to = (dst ^ (i << 6)) + 8 * g * L::kRowBytes;
-          copy16(to, ok ? k + i * 64 : k_base, ok);
-          copy16(to + L::kMatrix, ok ? v + i * 64 : v_base, ok);
+          const int bytes = 4 * i < n ? 16 : 0;
+          copy16((key_to ^ (i << 6) ^ (g & 1 ? L::kOddGroup : 0)) + 8 * g * L::kRowBytes, k + i * 64, bytes);
+          copy16((value_to ^ (i << 6)) + 8 * g * L::kRowBytes, v + i * 64, bytes);
         }
       }
       if (k8 && lane < L::kKeys) {
-        const int64_t ks = there ? page * a.key.s_page + slot * a.key.s_token + it.head * a.key.s_head : 0;
-        const int64_t vs = there ? page * a.value.s_page + slot * a.value.s_token + it.head * a.value.s_head : 0;
+        const int64_t ks = there ? a.key.scale_at(page, slot) : 0;
+        const int64_t vs = !there ? 0 : a.same_strides ? ks : a.value.scale_at(page, slot);
         const uint32_t to = extra_at + stage * L::kExtra + 16 + lane * 4;
-        copy4(to, a.key.scale + ks, there);
-        copy4(to + L::kKeys * 4, a.value.scale + vs, there);
+        copy4(to, ks_base + ks, there);
+        copy4(to + L::kKeys * 4, vs_base + vs, there);
       }
     }
     copy_commit();
@@ -680,9 +711,13 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   uint8_t* const queries = tiles + L::kQueryAt;
   const uint32_t tiles_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_tiles));
   const uint32_t extra_at = static_cast<uint32_t>(__cvta_generic_to_shared(my_extra));
-  const uint32_t copy_off = L::at(r0, c);
-  const uint32_t key_off = k8 && !kSplit ? L::at(lane & 15, lane >> 4) : L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
-  const uint32_t value_off = L::kMatrix + L::at(lane & 15, lane >> 4);
+  // Fragments of keys. 16 bits: keys 8 z + 0 .. 7 are the columns of product z of two. 8 bits: keys 4 i + 2 z
+  // and + 1, so that a thread's columns of both products are four neighbouring keys, as the transposing load
+  // of the values has them.
+  const int key_z = kSplit || !k8 ? lane >> 4 : lane >> 3 & 1, key_chunk = kSplit || !k8 ? lane >> 3 & 1 : lane >> 4;
+  const uint32_t key_off = L::key_at(k8 ? (lane & 6) * 2 + (lane & 1) + 2 * key_z : (lane & 7) + 8 * key_z, key_chunk);
+  const auto column = [&](int i, int e) { return k8 ? 16 * (i >> 1) + 4 * c + 2 * (i & 1) + e : 8 * i + 2 * c + e; };
+  const uint32_t value_off = L::kMatrix + L::at(lane & 15, lane >> 4);   // of values
   const int my_chunks = a.D * kElem / 16 - c;                      // chunks c, c + 4, .. that a row has
 
   const Range r = my_range(a);
@@ -706,7 +741,9 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     Feed<L, k8, kElem> feed{a, it, a.table.entry + b * a.table.stride,
                             static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem,
                             static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem,
-                            begin, end, count, my_extra, tiles_at, extra_at, copy_off, my_chunks, -1, 0};
+                            a.key.scale + it.head * a.key.s_head, a.value.scale + it.head * a.value.s_head,
+                            begin, end, count, my_extra, tiles_at, extra_at, L::key_at(r0, c),
+                            L::kMatrix + L::at(r0, c), my_chunks, -1, 0};
     feed.look_up(0);
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
@@ -720,7 +757,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       const int row = i / (kDP / 8), d = i % (kDP / 8) * 8;
       Raw<T, 8> piece{};
       if (row < rows && d < a.D) {
-        const int tt = row / it.heads, h = it.head * a.group + it.h0 + row - tt * it.heads;
+        const int tt = token_of(it, row), h = it.head * a.group + it.h0 + row - tt * it.heads;
         const T* const src = static_cast<const T*>(a.query) + b * a.q_batch + (it.t0 + tt) * a.q_token + h * a.q_head + d;
         if (a.q_wide) {
           piece = *reinterpret_cast<const Raw<T, 8>*>(src);
@@ -738,7 +775,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
     int row_token[kX];
 #pragma unroll
     for (int x = 0; x < kX; ++x) {
-      row_token[x] = (r0 + 8 * x) / it.heads;
+      row_token[x] = token_of(it, r0 + 8 * x);
       row_scale[x] = a.scale_log2;
     }
     if constexpr (!k8) {
@@ -829,7 +866,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       uint8_t* const values = my_tiles + stage * L::kStage + L::kMatrix;
       stage = stage == kStages - 1 ? 0 : stage + 1;
 
-      // p = queries x keys: columns 8 i + 2c, + 1 of rows r0 (0, 1) and r0 + 8 (2, 3). With 16 keys the sums
+      // p = queries x keys: column(i, 0) and column(i, 1) of rows r0 (0, 1) and r0 + 8 (2, 3). With 16 keys the sums
       // over the channels go in two, so that no chain of products is longer than four.
       constexpr int kChains = kGroups == 1 ? 2 : 1;
       float part[kChains][2 * kGroups][4];
@@ -886,8 +923,8 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           if (kSplit) p[i][e] += 0.0625f * (kChains == 2 ? part[0][i][e + 2] + part[kChains - 1][i][e + 2] : part[0][i][e + 2]);
         }
         if constexpr (k8) {
-          const float2 ks = *reinterpret_cast<const float2*>(extra + 16 + (8 * i + 2 * c) * 4);
-          const float2 vs = *reinterpret_cast<const float2*>(extra + 16 + (kKeys + 8 * i + 2 * c) * 4);
+          const float2 ks = *reinterpret_cast<const float2*>(extra + 16 + column(i, 0) * 4);
+          const float2 vs = *reinterpret_cast<const float2*>(extra + 16 + (kKeys + column(i, 0)) * 4);
           lv[i][0] = __log2f(vs.x);
           lv[i][1] = __log2f(vs.y);
 #pragma unroll
@@ -913,7 +950,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         for (int i = 0; i < 2 * kGroups; ++i)
 #pragma unroll
           for (int e = 0; e < kE; ++e)
-            if (!(on[e >> 1] >> (8 * i + 2 * c + (e & 1)) & 1)) p[i][e] = -INFINITY;
+            if (!(on[e >> 1] >> column(i, e & 1) & 1)) p[i][e] = -INFINITY;
       }
 
       // the running maximum of the logits (and of the logits with the values' scales)
@@ -979,31 +1016,30 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         for (; bad; bad &= bad - 1) {
           const int key = __ffs(bad) - 1, upto = it.p0 - j0 - key;          // p0 - j
 #pragma unroll
-          for (int i = 0; i < L::kChunks; ++i) {
-            uint32_t* const at_word = reinterpret_cast<uint32_t*>(values + L::at(key, i) + 4 * c);
-            const uint32_t word = *at_word, odd = not_finite<T, k8>(word);
+          for (int i = 0; i < kDP / 8; ++i) {                               // channels 8 i + 2c, + 1
+            using Two = typename RawOf<2 * kElem>::type;
+            Two* const two_at = reinterpret_cast<Two*>(values + L::at(key, i * 8 * kElem >> 4) + (i * 8 * kElem & 15) + 2 * c * kElem);
+            const uint32_t two = *two_at, odd = not_finite<T, k8>(two);
 #pragma unroll
             for (int x = 0; x < kX; ++x) {
               const int back = upto + row_token[x];                         // p - j
               if (back < 0 || back >= a.window) continue;
 #pragma unroll
-              for (int e = 0; e < 4 / kElem; ++e) {
+              for (int e = 0; e < 2; ++e) {
                 if (!(odd >> (8 * kElem * e) & 1)) continue;
                 float y = __int_as_float(0x7fc00000);
-                if (!k8) {
-                  y = as_float(bits_as<T>((uint16_t)(word >> (16 * e))));
-                }
-                acc[k8 ? 2 * i + (e & 1) : i][2 * x + (k8 ? e >> 1 : e)] += y;
+                if constexpr (!k8) y = as_float(bits_as<T>((uint16_t)(two >> (16 * e))));
+                acc[i][2 * x + e] += y;
               }
             }
             __syncwarp();
-            if (odd && r0 == 0) *at_word = word & ~odd;
+            if (odd && r0 == 0) *two_at = (Two)(two & ~odd);
           }
         }
         __syncwarp();
       }
 
-      // values: B fragments of two (8-bit: four) 8-channel columns for 16 keys at a time
+      // values: B fragments of 8-channel columns for 16 keys at a time
       const uint32_t vals = base + value_off;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
@@ -1016,17 +1052,13 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
             mma<M>(acc[2 * n + 1], w[g], f[2], f[3]);
           }
         } else {
-          // a 16-bit unit holds channels d, d + 1 of a key: sorted into pairs of keys for d and for d + 1
 #pragma unroll
           for (int n = 0; n < kSteps; n += 2) {
             uint32_t f[4];
-            ldmatrix4<true>(f, (vals ^ (n << 4)) + 16 * g * L::kRowBytes);
+            ldmatrix_bytes(f, (vals ^ (n << 4)) + 16 * g * L::kRowBytes);
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const uint32_t lo = f[2 * z], hi = f[2 * z + 1];
-              mma<M>(acc[2 * (n + z)], w[g], e4m3_to_f16(__byte_perm(lo, 0, 0x4420)), e4m3_to_f16(__byte_perm(hi, 0, 0x4420)));
-              mma<M>(acc[2 * (n + z) + 1], w[g], e4m3_to_f16(__byte_perm(lo, 0, 0x4431)), e4m3_to_f16(__byte_perm(hi, 0, 0x4431)));
-            }
+            for (int z = 0; z < 4; ++z)
+              mma<M>(acc[2 * n + z], w[g], e4m3_to_f16(f[z]), e4m3_to_f16(f[z] >> 16));
           }
         }
       }
@@ -1048,19 +1080,10 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       if (m[x] == -INFINITY) continue;                             // (not read)
       const float f = k8 ? ex2(mv[x] - m[x]) : 1.f;
       float* const dst = o + (warp * kRows + row) * o_stride;
-      if constexpr (!k8) {
 #pragma unroll
-        for (int i = 0; i < kDP / 8; ++i)
-          if (8 * i + 2 * c < a.D)
-            *reinterpret_cast<float2*>(dst + 8 * i + 2 * c) = make_float2(acc[i][2 * x], acc[i][2 * x + 1]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-          if (16 * i + 4 * c < a.D)
-            *reinterpret_cast<float4*>(dst + 16 * i + 4 * c) =
-                make_float4(f * acc[2 * i][2 * x], f * acc[2 * i + 1][2 * x], f * acc[2 * i][2 * x + 1],
-                            f * acc[2 * i + 1][2 * x + 1]);
-      }
+      for (int i = 0; i < kDP / 8; ++i)
+        if (8 * i + 2 * c < a.D)
+          *reinterpret_cast<float2*>(dst + 8 * i + 2 * c) = make_float2(f * acc[i][2 * x], f * acc[i][2 * x + 1]);
     }
     __syncthreads();
     const int part = part_of(a, r, item_begin, item_end, (int64_t)b * a.items + index);
@@ -1117,7 +1140,9 @@ decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
     Feed<L, k8, kElem> feed{a, it, a.table.entry + b * a.table.stride,
                             static_cast<const uint8_t*>(a.key.base) + it.head * a.key.head * kElem,
                             static_cast<const uint8_t*>(a.value.base) + it.head * a.value.head * kElem,
-                            begin, end, count, my_extra, tiles_at, extra_at, L::at(r0, c), my_chunks, -1, 0};
+                            a.key.scale + it.head * a.key.s_head, a.value.scale + it.head * a.value.s_head,
+                            begin, end, count, my_extra, tiles_at, extra_at, L::key_at(r0, c),
+                            L::kMatrix + L::at(r0, c), my_chunks, -1, 0};
     feed.look_up(0);
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
@@ -1129,7 +1154,7 @@ decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
       const int row = i / (kDP / 4), d = i % (kDP / 4) * 4;
       float4 piece = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < rows && d < a.D) {
-        const int tt = row / it.heads, h = it.head * a.group + it.h0 + row - tt * it.heads;
+        const int tt = token_of(it, row), h = it.head * a.group + it.h0 + row - tt * it.heads;
         const float* const src = static_cast<const float*>(a.query) + b * a.q_batch + (it.t0 + tt) * a.q_token + h * a.q_head + d;
         piece = a.q_wide ? *reinterpret_cast<const float4*>(src) : make_float4(src[0], src[1], src[2], src[3]);
       }
@@ -1140,7 +1165,7 @@ decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
     float acc[kRows][kPieces * kChannels], m[kRows], l[kRows];
 #pragma unroll
     for (int x = 0; x < kRows; ++x) {
-      row_token[x] = x / it.heads;
+      row_token[x] = token_of(it, x);
       m[x] = -INFINITY;
       l[x] = 0.f;
 #pragma unroll
@@ -1275,8 +1300,8 @@ decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
 
 // ---- the join --------------------------------------------------------------------------------------------
 // A warp per row of an item; items that one block had are done. A lane has a part's maximum and sum, then the
-// lanes share the channels.
-template <class T>
+// lanes share the channels, kN each.
+template <class T, int kN>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a,
                                                                int rows_max) {
   const int lane = threadIdx.x & 31;
@@ -1290,12 +1315,13 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
   const int2 covered = a.covered[id];
   if (covered.y <= 1) return;
   // the first block's part is its second one (the item began there), the others' their first
-  const auto slot = [&](int i) {
-    return (int64_t)(2 * (covered.x + i) + (i == 0 ? 1 : 0)) * rows_max + row;
-  };
-  float m = -INFINITY, l = 0.f, acc[8];
+  const auto slot = [&](int i) { return (2 * (covered.x + i) + (i == 0 ? 1 : 0)) * rows_max + row; };
+  constexpr int kMostPieces = 256 / (32 * kN);       // of a lane
+  float m = -INFINITY, l = 0.f, acc[kMostPieces][kN];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  for (int y = 0; y < kMostPieces; ++y)
+#pragma unroll
+    for (int e = 0; e < kN; ++e) acc[y][e] = 0.f;
   for (int i0 = 0; i0 < covered.y; i0 += 32) {
     const int count = min(32, covered.y - i0);
     const float2 p = lane < count ? a.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
@@ -1310,25 +1336,41 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
     for (int f = 16; f > 0; f >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, f);
     l = l * keep + sum;
     m = next;
+    const uint32_t there = __ballot_sync(0xffffffffu, p.x != -INFINITY);      // others were not written
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] *= keep;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const float f = __shfl_sync(0xffffffffu, w, i), top_i = __shfl_sync(0xffffffffu, p.x, i);
-      const float* o = a.part_o + slot(i0 + i) * a.D;
-      if (top_i == -INFINITY) continue;         // nothing was written
+    for (int y = 0; y < kMostPieces; ++y)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < a.D) acc[e] += f * o[lane + 32 * e];
+      for (int e = 0; e < kN; ++e) acc[y][e] *= keep;
+    // eight parts' loads under way together
+    for (int i = 0; i < count; i += 8) {
+#pragma unroll
+      for (int y = 0; y < kMostPieces; ++y) {
+        const int d = (lane + 32 * y) * kN;
+        Elements<float, kN> o[8];
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          o[z] = Elements<float, kN>{};
+          if ((there >> (i + z) & 1) && d < a.D)
+            o[z] = *reinterpret_cast<const Elements<float, kN>*>(a.part_o + (int64_t)slot(i0 + i + z) * a.D + d);
+        }
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          const float f = __shfl_sync(0xffffffffu, w, i + z);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) acc[y][e] += f * o[z].v[e];
+        }
+      }
     }
   }
-  const int t = it.t0 + row / it.heads, h = it.head * a.group + it.h0 + row % it.heads;
-  const int64_t at = ((int64_t)b * a.T + t) * a.Hq + h;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (lane + 32 * e < a.D)
-      static_cast<T*>(a.out)[at * a.D + lane + 32 * e] = from_float<T>(m == -INFINITY ? 0.f : acc[e] / l);
-  if (lane == 0 && a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+  for (int y = 0; y < kMostPieces; ++y) {
+    const int d = (lane + 32 * y) * kN;
+    if (d >= a.D) continue;
+    Elements<float, kN> x;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x.v[e] = acc[y][e];
+    write_row<T, kN>(a, it, row, d, m, l, x);
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
@@ -1487,7 +1529,8 @@ int run(const DecodeArgs& a, bool in_chunks, int cache_dtype, int rows_max, cuda
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  B200NA_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_join_kernel<T>, a, rows_max));
+  B200NA_CUDA_TRY(in_chunks ? cudaLaunchKernelEx(&cfg, decode_join_kernel<T, 4>, a, rows_max)
+                            : cudaLaunchKernelEx(&cfg, decode_join_kernel<T, 1>, a, rows_max));
   return B200NA_OK;
 }
 
@@ -1543,11 +1586,14 @@ extern "C" B200NA_API int b200na_na1d_decode(const void* query, const int64_t* q
   a.head_blocks = p.head_blocks;
   a.items = (uint32_t)p.items;
   a.parts = p.parts;
+  a.cluster = p.cluster;
   a.step = p.step;
   a.unit = p.unit;
+  while (1 << a.unit_log2 < a.unit) ++a.unit_log2;
+  while (1 << a.cluster_log2 < a.cluster) ++a.cluster_log2;
   a.q_wide = reinterpret_cast<uintptr_t>(query) % 16 == 0 && (a.q_batch | a.q_token | a.q_head) % (16 / elem_bytes(dtype)) == 0;
-  a.cluster = p.cluster;
-  a.same_strides = a.key.page == a.value.page && a.key.token == a.value.token;
+  a.same_strides = a.key.page == a.value.page && a.key.token == a.value.token &&
+                   a.key.s_page == a.value.s_page && a.key.s_token == a.value.s_token;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   a.covered = reinterpret_cast<int2*>(w);
   a.part_ml = reinterpret_cast<float2*>(w + p.covered_bytes);

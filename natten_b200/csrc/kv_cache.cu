@@ -4,7 +4,7 @@
 // keys and values in one launch. A group of lanes holds a whole row in registers, 16 bytes a lane and
 // access, so the largest magnitude of a row (for its 8-bit scale) is a few shuffles away and the row is
 // not read again. A block works on consecutive tokens of one sequence, so that a sequence's start and
-// count are read once a block and places need 32-bit arithmetic only; a thread has kRows rows in flight.
+// count are read once a block and places need 32-bit arithmetic only; a thread has a row or two in flight.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -13,7 +13,9 @@ namespace b200na {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 2;         // rows of keys and of values that a thread has in flight
+// Rows of keys and of values that a thread has in flight. Reading 8-bit prefixes (355 MB): one 70 us, two 74,
+// three 92, four 121: registers cost more threads than rows in flight give. Writing does not mind (20.7 us).
+constexpr int kRowsRead = 1, kRowsWritten = 2;
 
 struct MoveArgs {
   PagedPool pool[2];             // keys, values
@@ -48,8 +50,8 @@ template <class T, int kVec> __device__ __forceinline__ uint32_t largest_bits(co
 template <class T, class P, int kVec, bool kWrite>
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes_log2) {
   constexpr int kMost = kVec >= 8 ? 1 : kVec >= 4 ? 2 : 8;    // accesses a lane makes of one row, D <= 256
-  constexpr int kAtOnce = kMost == 8 ? 1 : kRows;
   constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
+  constexpr int kAtOnce = kMost == 8 ? 1 : kWrite ? kRowsWritten : kRowsRead;
   using In = Raw<T, kVec>;
   using Cached = Raw<P, kVec>;
   const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
       h[u] = row - tt * a.heads;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        at[u][w] = kWrite ? data[w] + tt * a.token[w] + h[u] * a.head[w] : data[w] + (int64_t)row * a.D;
+        at[u][w] = data[w] + (kWrite ? tt * a.token[w] + h[u] * a.head[w] : (int64_t)row * a.D);
         if (kWrite) {
 #pragma unroll
           for (int i = 0; i < kMost; ++i) {
@@ -116,12 +118,18 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       const int pg = page[u] >= 0 ? page[u] : 0;
+      int64_t off[2];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const PagedPool& pool = a.pool[w];
-        const int64_t off = pg * pool.page + slot[u] * pool.token + h[u] * pool.head;
-        cached[u][w] = static_cast<P*>(pool.base) + (w && a.same_strides ? cached[u][0] - static_cast<P*>(a.pool[0].base) : off + lane * kVec);
-        if (kScaled) scale_at[u][w] = pg * pool.s_page + slot[u] * pool.s_token + h[u] * pool.s_head;
+        if (w && a.same_strides) {
+          off[1] = off[0];
+          scale_at[u][1] = scale_at[u][0];
+        } else {
+          off[w] = pool.at(pg, slot[u]) + pool.head_at(h[u]) + lane * kVec;
+          if (kScaled) scale_at[u][w] = pool.scale_at(pg, slot[u]) + pool.scale_head_at(h[u]);
+        }
+        cached[u][w] = static_cast<P*>(pool.base) + off[w];
         if (!kWrite) {
           scale[u][w] = kScaled && page[u] >= 0 ? pool.scale[scale_at[u][w]] : 0.f;
 #pragma unroll
@@ -224,13 +232,15 @@ int launch(MoveArgs a, cudaStream_t stream) {
   int sms = 0;
   const int rc = sm_count_of_current_device(&sms);
   if (rc != B200NA_OK) return rc;
-  const int64_t round = (kThreads >> lanes_log2) * kRows, all = (int64_t)a.B * a.T * a.heads / round;
+  constexpr int kAtOnce = kWrite ? kRowsWritten : kRowsRead;
+  const int64_t round = (kThreads >> lanes_log2) * kAtOnce, all = (int64_t)a.B * a.T * a.heads / round;
   const int64_t rows = round * std::max<int64_t>(1, std::min<int64_t>(8, all / (8 * sms)));
   a.tokens = rows > a.heads ? (int)rows / a.heads : 1;
   a.tiles = (a.T + a.tokens - 1) / a.tokens;
   a.heads_magic = a.heads == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / a.heads) + (((uint64_t)1 << 32) % a.heads != 0);
   a.same_strides = a.pool[0].page == a.pool[1].page && a.pool[0].token == a.pool[1].token &&
-                   a.pool[0].head == a.pool[1].head;
+                   a.pool[0].head == a.pool[1].head && a.pool[0].s_page == a.pool[1].s_page &&
+                   a.pool[0].s_token == a.pool[1].s_token && a.pool[0].s_head == a.pool[1].s_head;
   const int64_t blocks = (int64_t)a.B * a.tiles;
   if (blocks > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   if (wide) move_kernel<T, P, kWide, kWrite><<<(unsigned)blocks, kThreads, 0, stream>>>(a, lanes_log2);

@@ -22,6 +22,18 @@ struct PagedPool {
   float* scale;                 // fp32 per token and head; nullptr when the pool is not 8-bit
   int64_t page, token, head;    // strides in elements
   int64_t s_page, s_token, s_head;
+  bool narrow;                  // all of them fit 31 bits: one multiply-add each
+
+  __device__ __forceinline__ int64_t at(int pg, int slot) const {
+    if (narrow) return (int64_t)pg * (int)page + (int64_t)slot * (int)token;
+    return pg * page + slot * token;
+  }
+  __device__ __forceinline__ int64_t scale_at(int pg, int slot) const {
+    if (narrow) return (int64_t)pg * (int)s_page + (int64_t)slot * (int)s_token;
+    return pg * s_page + slot * s_token;
+  }
+  __device__ __forceinline__ int64_t head_at(int h) const { return narrow ? (int64_t)h * (int)head : h * head; }
+  __device__ __forceinline__ int64_t scale_head_at(int h) const { return narrow ? (int64_t)h * (int)s_head : h * s_head; }
 };
 
 struct PageTable {
@@ -63,6 +75,9 @@ inline PagedPool paged_pool(const b200na_kv_cache& c, bool value) {
     p.s_token = one[1] ? 0 : f[1];
     p.s_head = one[2] ? 0 : f[2];
   }
+  p.narrow = true;
+  for (int64_t stride : {p.page, p.token, p.head, p.s_page, p.s_token, p.s_head})
+    p.narrow = p.narrow && stride >= 0 && stride <= 0x7fffffff;
   return p;
 }
 

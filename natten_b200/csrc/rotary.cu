@@ -17,7 +17,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;   // head_dim <= 256
 constexpr int kMostTokens = 16;  // of a block
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 6;
 
 struct RotaryArgs {
   const void* in[2];
