@@ -1412,7 +1412,7 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   if (p->item_tokens > T) p->item_tokens = T < 1 ? 1 : T;
   const int rows = p->item_tokens * p->item_heads;
   if (p->rows_max == 16 && rows <= 8) p->rows_max = 8;
-  else if (p->in_chunks && dtype == B200NA_F32 && rows <= 2) p->rows_max = 2;
+  else if (p->in_chunks && dtype == B200NA_F32 && rows <= 4) p->rows_max = rows <= 2 ? 2 : 4;
   p->token_blocks = (T + p->item_tokens - 1) / p->item_tokens;
   // a tile for each of a block's warps
   const int elem = elem_bytes(cache->dtype);
@@ -1503,8 +1503,9 @@ template <class T, bool k8, int kRows> int run_mma_rows(const DecodeArgs& a, cud
 template <class T>
 int run_tiles(const DecodeArgs& a, bool eight_bits, int rows_max, cudaStream_t s) {
   if constexpr (std::is_same<T, float>::value) {
-    if (eight_bits) return rows_max == 2 ? run_fma<true, 2>(a, s) : run_fma<true, 8>(a, s);
-    return rows_max == 2 ? run_fma<false, 2>(a, s) : run_fma<false, 8>(a, s);
+    if (eight_bits)
+      return rows_max == 2 ? run_fma<true, 2>(a, s) : rows_max == 4 ? run_fma<true, 4>(a, s) : run_fma<true, 8>(a, s);
+    return rows_max == 2 ? run_fma<false, 2>(a, s) : rows_max == 4 ? run_fma<false, 4>(a, s) : run_fma<false, 8>(a, s);
   } else {
     if (eight_bits) return rows_max == 8 ? run_mma_rows<T, true, 8>(a, s) : run_mma_rows<T, true, 16>(a, s);
     return rows_max == 8 ? run_mma_rows<T, false, 8>(a, s) : run_mma_rows<T, false, 16>(a, s);
