@@ -24,7 +24,7 @@ namespace b200na {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kMostParts = 2 * 148;   // blocks of the first launch: two per SM
+constexpr int kMostParts = 2 * 148;   // blocks that the GPU holds: two per SM
 constexpr int kClusterUnits = 40;     // units of an item that a block of a cluster takes at most (see make_plan)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -220,9 +220,9 @@ __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
   return r;
 }
 
-// How a segment (the block's part of an item) leaves: whole, or as part 0 (the item began in an earlier
-// block) or 1 of the block; 2: as the block's part of its cluster's item. The block that has the item's first unit notes which blocks the join has to
-// look at.
+// How a segment (the block's part of an item) leaves: whole (-1), as part 0 of the block (the item began in an
+// earlier one) or 1, or as the block's part of its cluster's item (2). The block that has the item's first unit
+// notes which blocks the join has to look at.
 __device__ __forceinline__ int part_of(const DecodeArgs& a, const Range& r, uint32_t item_begin,
                                        uint32_t item_end, int64_t item_id) {
   if (a.cluster) return a.cluster == 1 ? -1 : 2;
@@ -497,11 +497,15 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 // ---- tensor cores: fp16 / bf16 queries, 16-byte rows ---------------------------------------------------
 // A warp works alone on tiles of kKeys keys with copies of its own (cp.async, kStages tiles in flight), so
 // nothing waits for another warp before the item's end: 128 KB in flight per SM. The products are small next
-// to the bytes (16 rows are padded to the instruction's 16, 2 x 16 flops a cached element), so mma.sync on
-// fragments that ldmatrix takes out of the copied rows is enough; tcgen05 would want 128-row tiles and the
-// probabilities in shared memory or TMEM for the same bytes.
+// to the bytes (rows are padded to the instruction's 16: 2 x 16 flops a cached element), so mma.sync on
+// fragments that ldmatrix takes out of the copied rows is enough (a 16-key bf16 tile: 32 of them, 256 of the
+// 1365 cycles that its 8 KB take at the copy rate); tcgen05 would want 128-row tiles and the probabilities in
+// shared memory or TMEM for the same bytes. Measured: 64 sequences of 4 x 128 channels behind 2048 tokens, 259 MB
+// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 74 us (64 %: the conversions
+// and exponentials of a 32-key tile take about as many issue slots as its bytes take cycles).
 //
-// 8-bit rows are converted to fp16, which holds every e4m3 value, in registers. A key's scale multiplies its
+// Weights are rounded to the values' 16-bit type for the second product, like in the prefill kernels; maxima,
+// sums and outputs are fp32. 8-bit rows are converted to fp16, which holds every e4m3 value, in registers. A key's scale multiplies its
 // logits; a value's scale goes into its weight as 2^(s_j + log2 scale_j - m'), with a running maximum m' of
 // its own, so that the largest of these weights is 1 whatever the scales are and fp16 loses only what is
 // 2^-24 of it. Queries are multiplied by a power of two that brings the row's largest to [1, 2), exactly.
@@ -578,6 +582,9 @@ template <int kDP, int kElem, int kRows, bool k32> struct Tile {
   static constexpr int kRowBytes = kDP * kElem;
   static constexpr int kChunks = kRowBytes / 16;                   // of a row
   static constexpr int kKeys = tile_keys(kRowBytes, kElem);
+  // Two blocks of an SM with three tiles a warp under way. Two tiles: 64 sequences, window 2048 equal, 8-bit
+  // contexts 72.6 instead of 73.7 us, 256 sequences, window 512 59.6 instead of 55.9; three blocks with two tiles
+  // (registers capped at 168): equal, 73.8 and 56.1.
   static constexpr int kStages = 3;
   static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
   static constexpr int kStage = 2 * kMatrix;
@@ -1427,14 +1434,15 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   while (B * p->items * (most / p->unit + 1) > 0x7fffffff && p->unit <= most) p->unit *= 2;
   const int64_t units = B * p->items * (most / p->unit + 1);
   if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
-  p->parts = (int)(units < kMostParts ? (units < 1 ? 1 : units) : kMostParts);
+  const int held = p->in_chunks && D > 128 && elem > 1 ? kMostParts / 2 : kMostParts;   // (Tile::kBlocks)
+  p->parts = (int)(units < held ? (units < 1 ? 1 : units) : held);
   // Clusters of the largest size that leaves every block a place of its own, where a block's share is bounded.
   // Against ranges and their join (us): 64 sequences, 4 heads, window 2048 (33 units) 49.5 / 57.6, window 512
   // (9) 18.9 / 29.0; 1 sequence, window 2048 (33 over 8 blocks) 12.5 / 26.8; 4 sequences of 1000 to 8190 tokens (128
   // over 8) 23.0 / 33.3. Beyond, ranges are right: lengths may differ by more than what the join costs.
   const int64_t item_units = most / p->unit + 1, item_count = B * p->items;
   p->cluster = 1;
-  while (p->cluster < 8 && p->cluster < item_units && item_count * p->cluster * 2 <= kMostParts) p->cluster *= 2;
+  while (p->cluster < 8 && p->cluster < item_units && item_count * p->cluster * 2 <= held) p->cluster *= 2;
   if (item_units > kClusterUnits * p->cluster) p->cluster = 0;
   if (p->cluster) {
     p->covered_bytes = p->ml_bytes = p->o_bytes = 0;

@@ -338,3 +338,64 @@ def test_native_front_and_registered_operators_give_the_same(monkeypatch):
     nb.na1d_decode(q, c, table, n)
     nb.kv_cache_read(c, table, 5, dtype=dtype)
     assert L.launches == before + 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,heads", [(1, 2), (1, 24), (4, 8)])
+def test_an_8_bit_element_that_is_no_number(dtype, tokens, heads):
+    """A NaN in the pool itself: of a key it reaches the rows that attend it, of a value their channel."""
+    for where in ("key", "value"):
+        q, cache, table, n = _state(dtype, E4M3, [90, 90], tokens, heads, 2, 64, 16, seed=4)
+        good = nb.na1d_decode(q, cache, table, n, 40)
+        pool = getattr(cache, where)
+        for p in (89, 89 - 40 - tokens + 1):        # the newest token; the last one before all windows
+            pool.view(torch.uint8)[table[0, p // 16].long(), p % 16, 0, 5] = 0x7F
+        out, lse = nb.na1d_decode(q, cache, table, n, 40, return_lse=True)
+        hit = torch.zeros(2, tokens, heads, 64, dtype=torch.bool, device="cuda")
+        hit[0, -1, :heads // 2, slice(None) if where == "key" else 5] = True
+        assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], good[~hit])
+        assert torch.equal(torch.isnan(lse), hit.all(-1))
+
+
+def test_many_rows_and_ranges_of_wide_heads():
+    """Items of 16 rows over ranges and their join; heads that fill an SM's shared memory."""
+    for dtype, cache_dtype in TYPES:
+        _check(*_state(dtype, cache_dtype, [12000, 40], 1, 16, 1, 128, 64))
+        _check(*_state(dtype, cache_dtype, [9000, 500, 1], 3, 4, 1, 256, 64))
+
+
+FIRST_CALLS = """
+import torch
+import natten_b200 as nb
+torch.zeros(1, device="cuda")
+cache = nb.KVCache.allocate(8, 16, 2, 64, torch.float8_e4m3fn)
+table = torch.arange(8, device="cuda").int().view(1, 8)
+n = torch.full((1,), 100, dtype=torch.int32, device="cuda")
+q, k = torch.randn(1, 100, 4, 64, device="cuda").bfloat16(), torch.randn(1, 100, 2, 64, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a, b = nb.rotary(q, k)
+    nb.kv_cache_write(cache, b, b, table)
+    key, value = nb.kv_cache_read(cache, table, 100)
+    outs = [nb.na1d_decode(a[:, -t:], cache, table, n, w) for t in (1, 8) for w in (None, 40)]
+graph.replay()
+torch.cuda.synchronize()
+mine = [t.clone() for t in (a, b, key, value, *outs)]
+a, b = nb.rotary(q, k)
+nb.kv_cache_write(cache, b, b, table)
+again = [a, b, *nb.kv_cache_read(cache, table, 100)]
+again += [nb.na1d_decode(a[:, -t:], cache, table, n, w) for t in (1, 8) for w in (None, 40)]
+assert all(torch.equal(x, y) for x, y in zip(mine, again))
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """These kernels need no set-up of the device before they are recorded."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stdout + done.stderr

@@ -247,3 +247,32 @@ def test_native_front_and_registered_operators_give_the_same(monkeypatch):
     before = L.launches
     torch.autograd.grad((a, b), (q, k), (dq, dk))
     assert L.launches == before + 1
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("batch,sides,heads,heads_kv,dim", [
+    (70, (6, 50), 2, 1, 64),          # batch entries that share a block, the last group of them ragged
+    (33, (5, 9, 30), 3, 0, 48),
+    (64, (641,), 1, 1, 16),
+    (300, (1,), 2, 2, 32),
+])
+def test_batch_entries_share_their_angles(given, batch, sides, heads, heads_kv, dim):
+    torch.manual_seed(11)
+    q = torch.randn(batch, heads, *sides, dim).half().cuda().movedim(1, -2)
+    k = torch.randn(batch, *sides, heads_kv, dim).half().cuda() if heads_kv else None
+    at = ref.grid_positions(sides, [0] * len(sides))
+    kw = {}
+    if given:
+        at = torch.randint(0, 1000, (1, *sides, 2)).double()
+        kw = {"positions": at.int().cuda()}
+    dims = [2 * (dim // 8), 2 * (dim // 16), 0][:at.shape[-1]]       # the rest passes through
+    got = nb.rotary(q, k, dims, **kw)
+    theta, scale = [1e4] * len(dims), [1.0] * len(dims)
+    _check(q, got if k is None else got[0], dims, theta, scale, at, False)
+    if k is not None:
+        _check(k, got[1], dims, theta, scale, at, False)
+    # positions of each batch entry's own, the same ones: the same bits
+    if given:
+        own = nb.rotary(q, k, dims, positions=kw["positions"].expand(batch, *sides, 2))
+        for x, y in zip((got,) if k is None else got, (own,) if k is None else own):
+            assert torch.equal(x, y)
