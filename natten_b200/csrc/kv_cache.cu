@@ -4,7 +4,9 @@
 // keys and values in one launch. A group of lanes holds a whole row in registers, 16 bytes a lane and
 // access, so the largest magnitude of a row (for its 8-bit scale) is a few shuffles away and the row is
 // not read again. A block works on consecutive tokens of one sequence, so that a sequence's start and
-// count are read once a block and places need 32-bit arithmetic only; a thread has a row or two in flight.
+// count are read once a block and places need 32-bit arithmetic only. One row of keys and one of values to a
+// lane at a time: reading 8-bit prefixes (355 MB) takes 66 us so, 69 with two, 92 with three, 121 with four rows
+// in flight, whose registers cost more threads than they give; writing 8-bit prompts (63 MB) 16.7 us, 18.4 with two.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -13,9 +15,9 @@ namespace b200na {
 namespace {
 
 constexpr int kThreads = 256;
-// Rows of keys and of values that a thread has in flight. Reading 8-bit prefixes (355 MB): one 70 us, two 74,
-// three 92, four 121: registers cost more threads than rows in flight give. Writing does not mind (20.7 us).
-constexpr int kRowsRead = 1, kRowsWritten = 2;
+// Accesses of a row that a lane makes at least: two where the row has a scale, whose work is then shared by
+// twice as many elements.
+__host__ __device__ constexpr int lane_share(bool scaled, int vec) { return scaled && vec > 1 ? 2 : 1; }
 
 struct MoveArgs {
   PagedPool pool[2];             // keys, values
@@ -23,6 +25,7 @@ struct MoveArgs {
   PageTable table;
   void* data[2];                 // [B, T, heads, D]: given to the write, filled (contiguous) by the read
   int64_t batch[2], token[2], head[2];   // its strides (elements)
+  bool narrow;                   // those of tokens and heads fit 31 bits
   const int* start;
   const int* counts;
   int B, T, heads, D;
@@ -49,9 +52,8 @@ template <class T, int kVec> __device__ __forceinline__ uint32_t largest_bits(co
 // Lanes per row: a power of two that holds D / kVec accesses, 32 at most (then several each).
 template <class T, class P, int kVec, bool kWrite>
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes_log2) {
-  constexpr int kMost = kVec >= 8 ? 1 : kVec >= 4 ? 2 : 8;    // accesses a lane makes of one row, D <= 256
   constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
-  constexpr int kAtOnce = kMost == 8 ? 1 : kWrite ? kRowsWritten : kRowsRead;
+  constexpr int kMost = (kVec >= 8 ? 1 : kVec >= 4 ? 2 : 8) * lane_share(kScaled, kVec);   // accesses of one row, D <= 256
   using In = Raw<T, kVec>;
   using Cached = Raw<P, kVec>;
   const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
@@ -72,144 +74,129 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
     data[w] = static_cast<T*>(a.data[w]) + b * a.batch[w] + t0 * a.token[w] + lane * kVec;
   const int step = kVec << lanes_log2;                               // elements between a lane's accesses
   // (every lane of a warp takes part in every round: the shuffles below need them all)
-  for (int row0 = 0; row0 < rows; row0 += groups * kAtOnce) {
-    In x[kAtOnce][2][kMost];
-    bool live[kAtOnce];
-    int h[kAtOnce], slot[kAtOnce], page[kAtOnce];
-    T* at[kAtOnce][2];
+  for (int row0 = 0; row0 < rows; row0 += groups) {
+    const int row = row0 + group;
+    const bool live = row < rows;
+    const int tt = a.heads == 1 ? row : (int)__umulhi(row, a.heads_magic), h = row - tt * a.heads;
+    In x[2][kMost];
+    T* at[2];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int row = row0 + u * groups + group;
-      live[u] = row < rows;
-      const int tt = a.heads == 1 ? row : (int)__umulhi(row, a.heads_magic);
-      h[u] = row - tt * a.heads;
+    for (int w = 0; w < 2; ++w) {
+      at[w] = data[w] + (!kWrite ? (int64_t)row * a.D
+                         : a.narrow ? (int64_t)tt * (int)a.token[w] + (int64_t)h * (int)a.head[w]
+                                    : tt * a.token[w] + h * a.head[w]);
+      if (kWrite) {
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        at[u][w] = data[w] + (kWrite ? tt * a.token[w] + h[u] * a.head[w] : (int64_t)row * a.D);
-        if (kWrite) {
-#pragma unroll
-          for (int i = 0; i < kMost; ++i) {
-            x[u][w][i] = In{};
-            if (live[u] && mine(i)) x[u][w][i] = *reinterpret_cast<const In*>(at[u][w] + i * step);
-          }
+        for (int i = 0; i < kMost; ++i) {
+          x[w][i] = In{};
+          if (live && mine(i)) x[w][i] = *reinterpret_cast<const In*>(at[w] + i * step);
         }
-      }
-      page[u] = -1;
-      slot[u] = 0;
-      const int t = t0 + tt;
-      const int64_t p = start + t;
-      if (live[u] && t < count && p >= 0) {
-        uint32_t index = (uint32_t)p;                                // (start and t are 31 bits each)
-        if (a.table.shift >= 0) {
-          index >>= a.table.shift;
-          slot[u] = (uint32_t)p & (a.table.page_size - 1);
-        } else {
-          index /= (uint32_t)a.table.page_size;
-          slot[u] = (uint32_t)p - index * a.table.page_size;
-        }
-        if (index < (uint32_t)a.table.max_pages) page[u] = entries[index];
-        if ((uint32_t)page[u] >= (uint32_t)a.table.pages) page[u] = -1;
       }
     }
-    Cached y[kAtOnce][2][kMost];
-    float scale[kAtOnce][2];
-    int64_t scale_at[kAtOnce][2];
-    P* cached[kAtOnce][2];
+    int page = -1, slot = 0;
+    const int64_t p = start + t0 + tt;
+    if (live && t0 + tt < count && p >= 0) {
+      uint32_t index = (uint32_t)p;                                  // (start and t are 31 bits each)
+      if (a.table.shift >= 0) {
+        index >>= a.table.shift;
+        slot = (uint32_t)p & (a.table.page_size - 1);
+      } else {
+        index /= (uint32_t)a.table.page_size;
+        slot = (uint32_t)p - index * a.table.page_size;
+      }
+      if (index < (uint32_t)a.table.max_pages) page = entries[index];
+      if ((uint32_t)page >= (uint32_t)a.table.pages) page = -1;
+    }
+    const bool there = page >= 0;
+    Cached y[2][kMost];
+    float scale[2] = {0.f, 0.f};
+    int64_t off[2] = {0, 0}, scale_at[2] = {0, 0};
+    P* cached[2];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int pg = page[u] >= 0 ? page[u] : 0;
-      int64_t off[2];
+    for (int w = 0; w < 2; ++w) {
+      const PagedPool& pool = a.pool[w];
+      if (w && a.same_strides) {
+        off[1] = off[0];
+        scale_at[1] = scale_at[0];
+      } else if (there) {
+        off[w] = pool.at(page, slot) + pool.head_at(h) + lane * kVec;
+        if (kScaled) scale_at[w] = pool.scale_at(page, slot) + pool.scale_head_at(h);
+      }
+      cached[w] = static_cast<P*>(pool.base) + off[w];
+      if (!kWrite) {
+        if (kScaled && there) scale[w] = pool.scale[scale_at[w]];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const PagedPool& pool = a.pool[w];
-        if (w && a.same_strides) {
-          off[1] = off[0];
-          scale_at[u][1] = scale_at[u][0];
-        } else {
-          off[w] = pool.at(pg, slot[u]) + pool.head_at(h[u]) + lane * kVec;
-          if (kScaled) scale_at[u][w] = pool.scale_at(pg, slot[u]) + pool.scale_head_at(h[u]);
-        }
-        cached[u][w] = static_cast<P*>(pool.base) + off[w];
-        if (!kWrite) {
-          scale[u][w] = kScaled && page[u] >= 0 ? pool.scale[scale_at[u][w]] : 0.f;
-#pragma unroll
-          for (int i = 0; i < kMost; ++i) {
-            y[u][w][i] = Cached{};
-            if (page[u] >= 0 && mine(i)) y[u][w][i] = *reinterpret_cast<const Cached*>(cached[u][w] + i * step);
-          }
+        for (int i = 0; i < kMost; ++i) {
+          y[w][i] = Cached{};
+          if (there && mine(i)) y[w][i] = *reinterpret_cast<const Cached*>(cached[w] + i * step);
         }
       }
     }
     if constexpr (kWrite && kScaled) {
+      uint32_t most[2] = {0, 0};
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        uint32_t most[2] = {0, 0};
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int i = 0; i < kMost; ++i) most[w] = largest_bits<T, kVec>(x[w][i], most[w]);
+      if constexpr (sizeof(T) == 2) {
+        // keys in the low half, values in the high one
+        uint32_t both = __vmaxu2(__byte_perm(most[0], most[1], 0x5410), __byte_perm(most[0], most[1], 0x7632));
+        for (int o = 1; o < 1 << lanes_log2; o <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+        scale[0] = as_float(bits_as<T>((uint16_t)both));
+        scale[1] = as_float(bits_as<T>((uint16_t)(both >> 16)));
+      } else {
+        for (int o = 1; o < 1 << lanes_log2; o <<= 1)
 #pragma unroll
-          for (int i = 0; i < kMost; ++i) most[w] = largest_bits<T, kVec>(x[u][w][i], most[w]);
-        if constexpr (sizeof(T) == 2) {
-          // keys in the low half, values in the high one
-          uint32_t both = __vmaxu2(__byte_perm(most[0], most[1], 0x5410), __byte_perm(most[0], most[1], 0x7632));
-          for (int o = 1; o < 1 << lanes_log2; o <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
-          scale[u][0] = as_float(bits_as<T>((uint16_t)both));
-          scale[u][1] = as_float(bits_as<T>((uint16_t)(both >> 16)));
-        } else {
-          for (int o = 1; o < 1 << lanes_log2; o <<= 1)
+          for (int w = 0; w < 2; ++w) most[w] = max(most[w], __shfl_xor_sync(0xffffffffu, most[w], o));
+        scale[0] = __int_as_float(most[0]);
+        scale[1] = __int_as_float(most[1]);
+      }
 #pragma unroll
-            for (int w = 0; w < 2; ++w) most[w] = max(most[w], __shfl_xor_sync(0xffffffffu, most[w], o));
-          scale[u][0] = __int_as_float(most[0]);
-          scale[u][1] = __int_as_float(most[1]);
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          // most / 448, correctly rounded (a product and Markstein's correction by its remainder); a row that
-          // is not finite reads back as NaN
-          const float m = scale[u][w], q = m * (1.f / kE4m3Max);
-          const float s = fmaxf(__fmaf_rn(__fmaf_rn(-kE4m3Max, q, m), 1.f / kE4m3Max, q), kSmallestScale);
-          scale[u][w] = m < INFINITY ? s : __int_as_float(0x7fc00000);
-          if (page[u] >= 0 && lane == 0) a.pool[w].scale[scale_at[u][w]] = scale[u][w];
-        }
+      for (int w = 0; w < 2; ++w) {
+        // most / 448, correctly rounded (a product and Markstein's correction by its remainder); a row that
+        // is not finite reads back as NaN
+        const float m = scale[w], q = m * (1.f / kE4m3Max);
+        const float s = fmaxf(__fmaf_rn(__fmaf_rn(-kE4m3Max, q, m), 1.f / kE4m3Max, q), kSmallestScale);
+        scale[w] = m < INFINITY ? s : __int_as_float(0x7fc00000);
+        if (there && lane == 0) a.pool[w].scale[scale_at[w]] = scale[w];
       }
     }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u)
+    for (int w = 0; w < 2; ++w) {
+      float factor = 1.f;
+      if (kScaled) factor = kWrite ? __frcp_rn(scale[w]) : scale[w];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        float factor = 1.f;
-        if (kScaled) factor = kWrite ? __frcp_rn(scale[u][w]) : scale[u][w];
+      for (int i = 0; i < kMost; ++i) {
+        if constexpr (kWrite) {
+          if (!there || !mine(i)) continue;
+          if constexpr (kScaled) {
+            float f[kVec];
+            to_floats<T, kVec>(x[w][i], f);
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) {
-          if constexpr (kWrite) {
-            if (page[u] < 0 || !mine(i)) continue;
-            if constexpr (kScaled) {
+            for (int e = 0; e < kVec; ++e) f[e] *= factor;
+            y[w][i] = from_floats<P, kVec>(f);
+          } else {
+            y[w][i] = x[w][i];
+          }
+          *reinterpret_cast<Cached*>(cached[w] + i * step) = y[w][i];
+        } else {
+          if (!live || !mine(i)) continue;
+          if constexpr (kScaled) {
+            x[w][i] = In{};
+            if (there) {
               float f[kVec];
-              to_floats<T, kVec>(x[u][w][i], f);
+              to_floats<P, kVec>(y[w][i], f);
 #pragma unroll
               for (int e = 0; e < kVec; ++e) f[e] *= factor;
-              y[u][w][i] = from_floats<P, kVec>(f);
-            } else {
-              y[u][w][i] = x[u][w][i];
+              x[w][i] = from_floats<T, kVec>(f);
             }
-            *reinterpret_cast<Cached*>(cached[u][w] + i * step) = y[u][w][i];
           } else {
-            if (!live[u] || !mine(i)) continue;
-            if constexpr (kScaled) {
-              x[u][w][i] = In{};
-              if (page[u] >= 0) {
-                float f[kVec];
-                to_floats<P, kVec>(y[u][w][i], f);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) f[e] *= factor;
-                x[u][w][i] = from_floats<T, kVec>(f);
-              }
-            } else {
-              x[u][w][i] = y[u][w][i];
-            }
-            *reinterpret_cast<In*>(at[u][w] + i * step) = x[u][w][i];
+            x[w][i] = y[w][i];
           }
+          *reinterpret_cast<In*>(at[w] + i * step) = x[w][i];
         }
       }
+    }
   }
 }
 
@@ -226,17 +213,21 @@ int launch(MoveArgs a, cudaStream_t stream) {
   }
   const int accesses = wide ? a.D / kWide : a.D;
   int lanes_log2 = 0;
-  while (lanes_log2 < 5 && (1 << lanes_log2) < accesses) ++lanes_log2;
+  constexpr bool kScaled = std::is_same<P, __nv_fp8_e4m3>::value;
+  const int share = lane_share(kScaled, wide ? kWide : 1);
+  while (lanes_log2 < 5 && (share << lanes_log2) < accesses) ++lanes_log2;
   // Tokens of a block: rounds of its threads' rows, at least one token. More rounds (8 at most) share the wait
   // for the sequence's count and start, as long as every SM keeps eight blocks.
   int sms = 0;
   const int rc = sm_count_of_current_device(&sms);
   if (rc != B200NA_OK) return rc;
-  constexpr int kAtOnce = kWrite ? kRowsWritten : kRowsRead;
-  const int64_t round = (kThreads >> lanes_log2) * kAtOnce, all = (int64_t)a.B * a.T * a.heads / round;
+  const int64_t round = kThreads >> lanes_log2, all = (int64_t)a.B * a.T * a.heads / round;
   const int64_t rows = round * std::max<int64_t>(1, std::min<int64_t>(8, all / (8 * sms)));
   a.tokens = rows > a.heads ? (int)rows / a.heads : 1;
   a.tiles = (a.T + a.tokens - 1) / a.tokens;
+  a.narrow = true;
+  for (int w = 0; w < 2; ++w)
+    for (int64_t stride : {a.token[w], a.head[w]}) a.narrow = a.narrow && stride >= 0 && stride <= 0x7fffffff;
   a.heads_magic = a.heads == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / a.heads) + (((uint64_t)1 << 32) % a.heads != 0);
   a.same_strides = a.pool[0].page == a.pool[1].page && a.pool[0].token == a.pool[1].token &&
                    a.pool[0].head == a.pool[1].head && a.pool[0].s_page == a.pool[1].s_page &&
