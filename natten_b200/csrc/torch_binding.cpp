@@ -1533,13 +1533,13 @@ PyObject* py_na1d_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t need =
         lib.na1d_decode_workspace(B, T, Hq, &c.c, (int)table.size(1), kernel, dilation, dt);
     if (need < 0) check((int)need, "b200na_na1d_decode_workspace");
-    const Tensor workspace = at::empty({need}, q.options().dtype(at::kByte));
+    const Tensor workspace = need > 0 ? at::empty({need}, q.options().dtype(at::kByte)) : Tensor();
     check(lib.na1d_decode(q.data_ptr(), q.strides().data(), &c.c, out.data_ptr(),
                           want_lse ? lse.data_ptr<float>() : nullptr, B, T, Hq, dt, ints_of(table),
                           table.stride(0), (int)table.size(1), ints_of(lengths), kernel, dilation, scale,
-                          workspace.data_ptr(), stream_of(q)),
+                          need > 0 ? workspace.data_ptr() : nullptr, stream_of(q)),
           "b200na_na1d_decode");
-    launches += 2;
+    launches += need > 0 ? 2 : 1;
   }
   return wrap(out, lse, want_lse);
   END_HANDLE_TH_ERRORS

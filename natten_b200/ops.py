@@ -525,9 +525,10 @@ def na1d_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, key_scale
                                                      kernel_size, dilation, dt)
         if need < 0:
             _lib.check(int(need), "b200na_na1d_decode_workspace", kernel_launches=0)
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 0 else None
         _lib.check(_lib.lib.b200na_na1d_decode(
             _ptr(query), _lib.longs(query.stride()[:3]), ctypes.byref(cache), _ptr(out), _ptr(lse), B, T,
             Hq, dt, _ptr(table), table.stride(0), table.shape[1], _ptr(lengths), kernel_size, dilation,
-            float(scale), _ptr(workspace), _stream(query)), "b200na_na1d_decode", kernel_launches=2)
+            float(scale), _ptr(workspace), _stream(query)), "b200na_na1d_decode",
+            kernel_launches=2 if need > 0 else 1)
     return out, lse
