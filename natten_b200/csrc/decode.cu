@@ -584,7 +584,8 @@ template <int kDP, int kElem, int kRows, bool k32> struct Tile {
   static constexpr int kKeys = tile_keys(kRowBytes, kElem);
   // Two blocks of an SM with three tiles a warp under way. Two tiles: 64 sequences, window 2048 equal, 8-bit
   // contexts 72.6 instead of 73.7 us, 256 sequences, window 512 59.6 instead of 55.9; three blocks with two tiles
-  // (registers capped at 168): equal, 73.8 and 56.1.
+  // (registers capped at 168): equal, 73.8 and 56.1. The next tile's products with the keys ahead of this one's
+  // weights, which leaves one tile under way: 49.6, 75.5 and 60.0 instead of 49.2, 73.7 and 55.9.
   static constexpr int kStages = 3;
   static constexpr int kMatrix = kKeys * kRowBytes;                // bytes of a tile of keys, or of values
   static constexpr int kStage = 2 * kMatrix;
