@@ -192,7 +192,7 @@ int launch(RotaryArgs a, int vec, int sms, cudaStream_t stream) {
   const int slots = pairs >= vec ? kThreads / (pairs / vec) : kMostTokens;
   const int most = std::min(std::min(slots, kMostTokens), 32 * 1024 / (8 * std::max(pairs, 1)));
   a.block_tokens = 1;
-  while (a.block_tokens * 2 <= most &&
+  while (a.block_tokens * 2 <= most && a.block_tokens < a.batch_tokens &&
          (a.block_tokens * 2 <= std::min<int64_t>(per, 16) ||
           (a.block_tokens * std::max(a.heads[0], a.heads[1]) < slots && a.block_tokens * 2 <= per * 8)))
     a.block_tokens *= 2;

@@ -46,9 +46,14 @@ class KVCache(NamedTuple):
         return cls(*pools)
 
 
+def _expect_cache(cache: KVCache) -> None:
+    if not isinstance(cache, KVCache):
+        raise ValueError(f"Expected a KVCache, got {type(cache)}.")
+
+
 def _check_cache(cache: KVCache) -> None:
     key, value, *scales = cache
-    if not isinstance(key, Tensor) or key.dim() != 4 or value.shape != key.shape:
+    if not isinstance(key, Tensor) or not isinstance(value, Tensor) or key.dim() != 4 or value.shape != key.shape:
         raise ValueError("A cache's pools are [pages, page_size, heads_kv, head_dim], keys and values "
                          "alike.")
     if key.dtype != value.dtype or key.device != value.device:
@@ -125,6 +130,7 @@ def kv_cache_write(cache: KVCache, key: Tensor, value: Tensor, page_table: Tenso
     Positions that are negative, behind the table, or on a table entry outside ``[0, pages)`` are dropped.
     The slots of one call must be different ones: of two tokens on the same slot, which one (or a mixture)
     is left is undefined."""
+    _expect_cache(cache)
     if (_native_eligible()
             and _native.kv_cache_write(cache, key, value, page_table, start, counts) is not None):
         return
@@ -153,8 +159,10 @@ def kv_cache_read(cache: KVCache, page_table: Tensor, length: int, start: Option
     Row t of sequence b is the token at ``start[b] + t`` (``t`` without ``start``); rows ``t >= counts[b]``
     and tokens that are on no page are zeros. ``dtype`` is the cache's, or fp32, fp16 or bf16 for an 8-bit
     cache (default bf16)."""
+    _expect_cache(cache)
     if dtype is None:
-        dtype = torch.bfloat16 if cache.key.dtype == torch.float8_e4m3fn else cache.key.dtype
+        dtype = getattr(cache.key, "dtype", None)
+        dtype = torch.bfloat16 if dtype == torch.float8_e4m3fn else dtype
     if _native_eligible():
         result = _native.kv_cache_read(cache, page_table, length, start, counts, dtype)
         if result is not None:
@@ -188,6 +196,7 @@ def na1d_decode(query: Tensor, cache: KVCache, page_table: Tensor, lengths: Tens
 
     The cache has the query's data type or is an 8-bit one. Returns the output in the query's type, with
     ``return_lse`` also the logsumexp (fp32 ``[batch, tokens, heads]``), as `merge_attentions` takes them."""
+    _expect_cache(cache)
     if _native_eligible():
         result = _native.na1d_decode(query, cache, page_table, lengths, kernel_size, dilation, scale,
                                      bool(return_lse))

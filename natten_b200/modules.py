@@ -17,7 +17,7 @@ from torch.nn.modules.module import _has_any_global_hook
 from . import _native
 from .checks import check_all_args
 from .functional import _native_eligible, attention, neighborhood_attention_generic
-from .kv_cache import KVCache, kv_cache_write, na1d_decode
+from .kv_cache import KVCache, _refuse_grad, kv_cache_write, na1d_decode
 from .positions import check_rotary_args, rotary
 
 
@@ -33,6 +33,11 @@ class NeighborhoodAttentionGeneric(nn.Module):
     Input and output are ``[batch, *token_layout, embed_dim]``. With ``rotary_theta`` queries and keys
     get rotary positions over the token axes (`rotary`: ``rotary_axis_dims`` channels each, neighbouring
     channels paired with ``rotary_interleaved``)."""
+
+    # (also for modules that were pickled without them)
+    rotary_theta: Any = None
+    rotary_axis_dims: Optional[Sequence[int]] = None
+    rotary_interleaved = False
 
     def __init__(self, na_dim: int, embed_dim: int, num_heads: int, kernel_size: Any,
                  stride: Any = 1, dilation: Any = 1, is_causal: Any = False, qkv_bias: bool = True,
@@ -125,16 +130,18 @@ class NeighborhoodAttention1D(NeighborhoodAttentionGeneric):
                 counts: Optional[Tensor] = None) -> Tensor:
         """The layer on whole prompts ``[batch, tokens, embed_dim]``, whose keys and values go into the
         cache: token t of sequence b at position t, if ``t < counts[b]`` (prompts padded at their end;
-        all without ``counts``). The rows of the output behind a prompt mean nothing."""
+        all without ``counts``). The rows of the output behind a prompt mean nothing. A dilated layer needs
+        as many tokens as its window spans, like `forward`."""
         self._check_serving(x)
         q, k, v = self._project(x)
-        kv_cache_write(cache, k, v, page_table, None, counts)
+        _refuse_grad("prefill()", q, k, v)
         if x.shape[1] < self.kernel_size[0] and self.dilation[0] == 1:      # a window over all of it
             out = attention(q, k, v, is_causal=True, scale=self.scale)
         else:
             out = neighborhood_attention_generic(q, k, v, kernel_size=self.kernel_size, stride=1,
                                                  dilation=self.dilation, is_causal=self.is_causal,
                                                  scale=self.scale)
+        kv_cache_write(cache, k, v, page_table, None, counts)
         return self.proj_drop(self.proj(out.reshape(x.shape)))
 
     def decode(self, x: Tensor, cache: KVCache, page_table: Tensor, lengths: Tensor) -> Tensor:

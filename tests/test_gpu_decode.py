@@ -72,6 +72,8 @@ TYPES = [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.
     ([150, 31], 1, 4, 2, 16, 16, None, 1),
     ([150, 31], 2, 2, 2, 208, 16, 90, 1),
     ([64, 31], 17, 2, 2, 32, 8, 20, 1),                                       # more queries than a window
+    ([70, 12], 2, 4, 4, 64, 1, 30, 1),                                        # pages of one token
+    ([300], 1, 4, 2, 128, 1024, None, 2),                                     # one page, dilated, all of it
 ])
 def test_shapes(dtype, cache_dtype, lengths, tokens, heads, heads_kv, dim, page, kernel_size, dilation):
     _check(*_state(dtype, cache_dtype, lengths, tokens, heads, heads_kv, dim, page), kernel_size, dilation)

@@ -16,6 +16,14 @@ def test_layer_arguments():
             nb.NeighborhoodAttention2D(64, 2, 5, **kw)
 
 
+def test_modules_pickled_before_there_were_positions():
+    layer = nb.NeighborhoodAttention2D(64, 2, 5)
+    state = {n: v for n, v in layer.__dict__.items() if not n.startswith("rotary")}
+    old = nb.NeighborhoodAttention2D.__new__(nb.NeighborhoodAttention2D)
+    old.__dict__.update(state)
+    assert repr(old) == repr(layer) and old.rotary_theta is None
+
+
 def test_serving_refusals():
     x = torch.zeros(2, 3, 64)
     cache = nb.KVCache.allocate(4, 8, 2, 32, torch.float32, device="cpu")
@@ -103,6 +111,22 @@ def test_prompt_and_steps_give_what_the_whole_sequence_gives(dtype, cache_dtype,
             for b in range(B):
                 end = int(at[b])
                 assert (y[b].float() - want[b, end - tokens:end].float()).abs().max() <= tol
+
+
+@pytest.mark.gpu
+def test_a_refused_prompt_leaves_the_cache_alone():
+    layer = nb.NeighborhoodAttention1D(64, 2, 7, 1, 4, True).cuda().half().eval()
+    cache = nb.KVCache.allocate(4, 8, 2, 32, torch.float16)
+    for t in cache[:2]:
+        t.zero_()
+    table = torch.arange(4, device="cuda").int().view(1, 4)
+    with torch.no_grad():
+        with pytest.raises(ValueError):
+            layer.prefill(torch.randn(1, 20, 64, device="cuda").half(), cache, table)      # 7 x 4 tokens
+        with pytest.raises(ValueError):
+            layer.decode(torch.randn(1, 1, 64, device="cuda").half(), cache, table,
+                         torch.ones(1, dtype=torch.int64, device="cuda"))
+    assert not cache.key.any() and not cache.value.any()
 
 
 @pytest.mark.gpu

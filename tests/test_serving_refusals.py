@@ -69,6 +69,8 @@ def test_cache_refusals():
         nb.KVCache(c.key.to(torch.float8_e4m3fn), c.value.to(torch.float8_e4m3fn)),
         nb.KVCache(c.key, c.value, torch.zeros(4, 8, 2), torch.zeros(4, 8, 2)),
         nb.KVCache(c.key[:, :0], c.value[:, :0]),
+        (c.key, c.value),
+        nb.KVCache(c.key, None),
     ]
     for bad in bad_caches:
         for call in (lambda: nb.kv_cache_write(bad, kv, kv, t), lambda: nb.kv_cache_read(bad, t, 3),
