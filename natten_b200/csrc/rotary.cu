@@ -41,7 +41,8 @@ struct RotaryArgs {
 template <class T, int kVec, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   // Rows that a thread has under way: about 96 bytes. A training step on 15 x 30 x 52 tokens of 12 + 12 heads
-  // with 1, 2, 3, 4, 6 rows of 16 bytes: 78, 64, 67, 68, 60 us.
+  // with 1, 2, 3, 4, 6 rows of 16 bytes: 78, 64, 67, 68, 60 us (58 now; a video of 32 x 48 x 80 tokens, 24 + 24 heads
+  // of 128 channels, 3.0 GB: 461 us, the copy rate).
   constexpr int kRowBytes = 2 * kVec * (int)sizeof(T), kUnroll = kRowBytes >= 32 ? 3 : 6;
   extern __shared__ __align__(16) float cs[];                 // [block_tokens][cosines, sines][stride]
   __shared__ int64_t in_at[2][kMostTokens], out_at[2][kMostTokens];   // offsets of the tokens' first head
@@ -51,6 +52,13 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int64_t token0 = (int64_t)(blockIdx.x - group * a.tiles) * block_tokens;
   const int b0 = group * a.block_batches, batches = min(a.block_batches, a.B - b0);
   const int count = (int)(a.batch_tokens - token0 < block_tokens ? a.batch_tokens - token0 : block_tokens);
+
+  // For the angles a thread keeps its pair: a launch parameter that every lane reads elsewhere is read one lane
+  // after the other, so it is read once.
+  const int at_once = pairs > 0 ? kThreads / pairs : 0, my_token = pairs > 0 ? threadIdx.x / pairs : 0;
+  const int my_pair = threadIdx.x - my_token * pairs;
+  const int my_axis = (my_pair >= a.first_pair[1] && a.axes > 1) + (my_pair >= a.first_pair[2] && a.axes > 2);
+  const double my_turns = my_token < at_once ? a.turns[my_pair] : 0.0;
 
   if ((int)threadIdx.x < count) {
     const int tt = threadIdx.x;
@@ -82,14 +90,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < count * pairs; i += kThreads) {
-    const int tt = i / pairs, pair = i - tt * pairs;
-    const int axis = (pair >= a.first_pair[1] && a.axes > 1) + (pair >= a.first_pair[2] && a.axes > 2);
-    const double turn = place[tt][axis] * a.turns[pair];
-    float s, c;
-    sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
-    cs[2 * tt * stride + pair] = c;
-    cs[(2 * tt + 1) * stride + pair] = s;
+  if (at_once > 0 && my_token < at_once) {
+    for (int t = my_token; t < count; t += at_once) {
+      const double turn = place[t][my_axis] * my_turns;
+      float s, c;
+      sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
+      cs[2 * t * stride + my_pair] = c;
+      cs[(2 * t + 1) * stride + my_pair] = s;
+    }
   }
   __syncthreads();
 
@@ -187,17 +195,19 @@ template <class T, bool kInterleaved>
 int launch(RotaryArgs a, int vec, int sms, cudaStream_t stream) {
   const int pairs = a.first_pair[a.axes], heads = a.heads[0] + a.heads[1];
   // Tokens of a block, a power of two so that a token's columns fill whole warps: as many as give each of its
-  // threads a row, while every SM has a block; more, as long as every SM has eight.
+  // threads a row, while every SM has a block; more, as long as every SM has eight. (21 x 31 x 96 tokens of 4 + 2
+  // heads with at most 8, 16, 32 tokens: 88, 60, 53 us; 44 now.)
   const int64_t tokens = a.B * a.batch_tokens, per = tokens / ((int64_t)sms * 8);
   const int slots = pairs >= vec ? kThreads / (pairs / vec) : kMostTokens;
   const int most = std::min(std::min(slots, kMostTokens), 32 * 1024 / (8 * std::max(pairs, 1)));
   a.block_tokens = 1;
   while (a.block_tokens * 2 <= most && a.block_tokens < a.batch_tokens &&
-         (a.block_tokens * 2 <= std::min<int64_t>(per, 16) ||
+         (a.block_tokens * 2 <= per ||
           (a.block_tokens * std::max(a.heads[0], a.heads[1]) < slots && a.block_tokens * 2 <= per * 8)))
     a.block_tokens *= 2;
   // Batch entries whose tokens stand at the same places share the angles: up to 32 rows of a token together.
-  // (16 videos of 6 + 3 heads 214 -> 195 us.)
+  // (16 videos of 6 + 3 heads 214 -> 195 us, 184 with the
+  // frequencies read once.)
   a.block_batches = 1;
   if (!a.positions || !a.positions_batched)
     while (a.block_batches < a.B && a.block_batches * 2 * heads <= 32 && a.block_batches * 2 * a.block_tokens <= per)
