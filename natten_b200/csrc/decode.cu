@@ -526,6 +526,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {      // of a scale: 2^-126 at least, or 0 where there is no key
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -933,8 +938,8 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         if constexpr (k8) {
           const float2 ks = *reinterpret_cast<const float2*>(extra + 16 + column(i, 0) * 4);
           const float2 vs = *reinterpret_cast<const float2*>(extra + 16 + (kKeys + column(i, 0)) * 4);
-          lv[i][0] = __log2f(vs.x);
-          lv[i][1] = __log2f(vs.y);
+          lv[i][0] = lg2(vs.x);
+          lv[i][1] = lg2(vs.y);
 #pragma unroll
           for (int e = 0; e < kE; ++e) p[i][e] *= e & 1 ? ks.y : ks.x;
         }
@@ -958,7 +963,10 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         for (int i = 0; i < 2 * kGroups; ++i)
 #pragma unroll
           for (int e = 0; e < kE; ++e)
-            if (!(on[e >> 1] >> column(i, e & 1) & 1)) p[i][e] = -INFINITY;
+            if (!(on[e >> 1] >> column(i, e & 1) & 1)) {
+              p[i][e] = -INFINITY;
+              if (k8 && kX == 1) lv[i][e & 1] = 0.f;               // left out, whatever its scale is
+            }
       }
 
       // the running maximum of the logits (and of the logits with the values' scales)
@@ -1007,7 +1015,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           const float ex = ex2(fmaf(p[i][e], row_scale[x], -base_m[x]));
           l[x] += ex;
           y[e] = k8 ? ex2(fmaf(p[i][e], row_scale[x], lv[i][e & 1]) - base_v[x]) : ex;
-          if (k8 && p[i][e] == -INFINITY) y[e] = 0.f;              // left out, whatever its scale is
+          if (k8 && kX == 2 && p[i][e] == -INFINITY) y[e] = 0.f;   // (two rows share the scale)
         }
         w[i >> 1][2 * (i & 1)] = Half2Of<M>::pack(y[0], y[1]);
         w[i >> 1][2 * (i & 1) + 1] = Half2Of<M>::pack(y[2], y[3]);
