@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 // fragments that ldmatrix takes out of the copied rows is enough (a 16-key bf16 tile: 32 of them, 256 of the
 // 1365 cycles that its 8 KB take at the copy rate); tcgen05 would want 128-row tiles and the probabilities in
 // shared memory or TMEM for the same bytes. Measured: 64 sequences of 4 x 128 channels behind 2048 tokens, 259 MB
-// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 74 us (64 %: the conversions
+// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 71 us (67 %: the conversions
 // and exponentials of a 32-key tile take about as many issue slots as its bytes take cycles).
 //
 // Weights are rounded to the values' 16-bit type for the second product, like in the prefill kernels; maxima,
@@ -570,11 +570,10 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two e4m3 values (low 16 bits) -> two fp16 values
-__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t x) {
-  uint32_t y;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
-  return y;
+// Four e4m3 values -> two fp16 values each, the low ones and the high ones.
+__device__ __forceinline__ void e4m3_to_f16(uint32_t x, uint32_t& low, uint32_t& high) {
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+      : "=r"(low), "=r"(high) : "r"(x));
 }
 
 // Keys of a warp's tile: about 4 KB of them, for cached elements of `elem` bytes.
@@ -921,8 +920,11 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
             ldmatrix4<false>(f, (keys ^ (k << 4)) + 16 * g * L::kRowBytes);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-              mma<M>(part[z % kChains][2 * g], q[k + z], e4m3_to_f16(f[2 * z]), e4m3_to_f16(f[2 * z] >> 16));
-              mma<M>(part[z % kChains][2 * g + 1], q[k + z], e4m3_to_f16(f[2 * z + 1]), e4m3_to_f16(f[2 * z + 1] >> 16));
+              uint32_t low, high;
+              e4m3_to_f16(f[2 * z], low, high);
+              mma<M>(part[z % kChains][2 * g], q[k + z], low, high);
+              e4m3_to_f16(f[2 * z + 1], low, high);
+              mma<M>(part[z % kChains][2 * g + 1], q[k + z], low, high);
             }
           }
       }
@@ -1073,8 +1075,11 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
             uint32_t f[4];
             ldmatrix_bytes(f, (vals ^ (n << 4)) + 16 * g * L::kRowBytes);
 #pragma unroll
-            for (int z = 0; z < 4; ++z)
-              mma<M>(acc[2 * n + z], w[g], e4m3_to_f16(f[z]), e4m3_to_f16(f[z] >> 16));
+            for (int z = 0; z < 4; ++z) {
+              uint32_t low, high;
+              e4m3_to_f16(f[z], low, high);
+              mma<M>(acc[2 * n + z], w[g], low, high);
+            }
           }
         }
       }
