@@ -220,6 +220,12 @@ __device__ __forceinline__ Range my_range(const DecodeArgs& a) {
   return r;
 }
 
+// The join's blocks may take their places as blocks of this launch end (they wait for all of it before they read
+// anything; every block of this launch has its place from the start).
+__device__ __forceinline__ void allow_join(const DecodeArgs& a) {
+  if (!a.cluster) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // How a segment (the block's part of an item) leaves: whole (-1), as part 0 of the block (the item began in an
 // earlier one) or 1, or as the block's part of its cluster's item (2). The block that has the item's first unit
 // notes which blocks the join has to look at.
@@ -365,6 +371,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
   __shared__ float2 ml[kWarps * kRows], joint_ml[kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Range r = my_range(a);
+  allow_join(a);
   int b = r.b, length = r.length;
   uint32_t before = r.before;
   for (uint32_t at = r.begin; at < r.end;) {
@@ -733,6 +740,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   const int my_chunks = a.D * kElem / 16 - c;                      // chunks c, c + 4, .. that a row has
 
   const Range r = my_range(a);
+  allow_join(a);
   int b = r.b, length = r.length;
   uint32_t before = r.before;
   for (uint32_t at = r.begin; at < r.end;) {
@@ -1142,6 +1150,7 @@ decode_fma_kernel(const __grid_constant__ DecodeArgs a) {
   const int my_chunks = a.D * kElem / 16 - c;
 
   const Range r = my_range(a);
+  allow_join(a);
   int b = r.b, length = r.length;
   uint32_t before = r.before;
   for (uint32_t at = r.begin; at < r.end;) {
@@ -1539,8 +1548,6 @@ int run(const DecodeArgs& a, bool in_chunks, int cache_dtype, int rows_max, cuda
   int rc = in_chunks ? run_tiles<T>(a, cache_dtype == B200NA_E4M3, rows_max, s)
            : cache_dtype == B200NA_E4M3 ? run_simt<T, __nv_fp8_e4m3>(a, rows_max, s) : run_simt<T, T>(a, rows_max, s);
   if (rc != B200NA_OK || a.cluster) return rc;
-  // The join's blocks may take their places while the first launch's last ones run (they wait for its end
-  // before they read anything).
   cudaLaunchConfig_t cfg{};
   const int64_t warps = (int64_t)a.B * a.items * rows_max;
   const int64_t blocks = (warps + kWarps - 1) / kWarps;
