@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 // fragments that ldmatrix takes out of the copied rows is enough (a 16-key bf16 tile: 32 of them, 256 of the
 // 1365 cycles that its 8 KB take at the copy rate); tcgen05 would want 128-row tiles and the probabilities in
 // shared memory or TMEM for the same bytes. Measured: 64 sequences of 4 x 128 channels behind 2048 tokens, 259 MB
-// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 71 us (67 %: the conversions
+// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 70 us (68 %: the conversions
 // and exponentials of a 32-key tile take about as many issue slots as its bytes take cycles).
 //
 // Weights are rounded to the values' 16-bit type for the second product, like in the prefill kernels; maxima,
