@@ -830,7 +830,8 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           row_scale[x] *= __int_as_float((127 - kUp + e) << 23);
         }
         if constexpr (kSplit) {
-          if (!(most < INFINITY)) row_scale[x] = __int_as_float(0x7fc00000);    // e4m3 has no infinity
+          // e4m3 has no infinity: NaNs in its place, which only the tokens that the row attends bring to it
+          if (!(most < INFINITY)) factor = __int_as_float(0x7fc00000);
           // A bf16 number is the sum of two e4m3 ones: the nearest one and what is left (four bits and sign,
           // times 16). Row r0 of the instruction is the first, row r0 + 8 the second.
 #pragma unroll
