@@ -49,6 +49,45 @@ template <class T, int kVec> __device__ __forceinline__ uint32_t largest_bits(co
   }
 }
 
+// The bytes of x / scale as the definition has them: a 32-bit division, then the rounding to e4m3. (A product with
+// the rounded reciprocal may leave the middle of two e4m3 numbers and end at the other one.) Two values an instruction.
+//  - 16-bit values: a product with the reciprocal in two parts, rounded once, 2^-45 off before that. The bytes are the
+//    division's for every pair of a 16-bit value and the largest magnitude of its row (all mantissas of fp16 and bf16,
+//    and the exponents at both ends of the range, were gone through).
+//  - fp32: the correctly rounded quotient by a product with the reciprocal and Markstein's correction by its remainder.
+//    Small scales and their rows are multiplied by 2^64 first, so that the remainders of all quotients that e4m3 does
+//    not round to zero are representable.
+// Writing 8-bit prompts out of 16-bit values (63 MB) takes 16.6 us so, as with the rounded reciprocal alone, and 17.1
+// with Markstein's correction; out of fp32 values (105 MB) 30.6 us, 28.9 with the reciprocal alone.
+template <class T> struct Quotient {
+  float2 up, over, factor;
+  __device__ __forceinline__ explicit Quotient(float scale) {
+    if constexpr (sizeof(T) == 2) {
+      const float r = __frcp_rd(scale), rest = __fmaf_rn(-scale, r, 1.f) * r;      // (never negative: -0 stays -0)
+      factor = make_float2(r, r);
+      up = make_float2(rest, rest);
+    } else {
+      const float u = scale < 0x1p-64f ? 0x1p64f : 1.f, r = __frcp_rn(scale * u);
+      up = make_float2(-u, -u);
+      over = make_float2(scale * u, scale * u);
+      factor = make_float2(-r, -r);
+    }
+  }
+  __device__ __forceinline__ float2 operator()(float2 x) const {
+    if constexpr (sizeof(T) == 2) return __ffma2_rn(x, factor, __fmul2_rn(x, up));
+    const float2 v = __fmul2_rn(x, up), q = __fmul2_rn(v, factor);                  // -x, x / scale
+    return __ffma2_rn(__ffma2_rn(over, q, v), factor, q);
+  }
+  template <int kN> __device__ __forceinline__ void divide(float (&x)[kN]) const {
+#pragma unroll
+    for (int e = 0; e < kN; e += 2) {
+      const float2 y = (*this)(make_float2(x[e], e + 1 < kN ? x[e + 1] : 0.f));
+      x[e] = y.x;
+      if (e + 1 < kN) x[e + 1] = y.y;
+    }
+  }
+};
+
 // Lanes per row: a power of two that holds D / kVec accesses, 32 at most (then several each).
 template <class T, class P, int kVec, bool kWrite>
 __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ MoveArgs a, int lanes_log2) {
@@ -163,8 +202,8 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      float factor = 1.f;
-      if (kScaled) factor = kWrite ? __frcp_rn(scale[w]) : scale[w];
+      const float factor = scale[w];
+      const Quotient<T> by(scale[w]);
 #pragma unroll
       for (int i = 0; i < kMost; ++i) {
         if constexpr (kWrite) {
@@ -172,8 +211,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
           if constexpr (kScaled) {
             float f[kVec];
             to_floats<T, kVec>(x[w][i], f);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) f[e] *= factor;
+            by.divide(f);
             y[w][i] = from_floats<P, kVec>(f);
           } else {
             y[w][i] = x[w][i];

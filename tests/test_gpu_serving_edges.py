@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import natten_b200 as nb
-from test_gpu_decode import TYPES, _state
+import serving_reference as ref
+from test_gpu_decode import E4M3, TYPES, _check, _state
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,35 @@ def test_an_infinite_query_that_attends_nothing(dtype, cache_dtype, heads):
         assert torch.isnan(out[2, 0, 0]).all()
         out[2, 0, 0], lse[2, 0, 0] = good[2, 0, 0], good_lse[2, 0, 0]
         assert torch.equal(out, good) and torch.equal(lse, good_lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_eight_bit_rows_are_divided_by_their_scale(dtype):
+    """The bytes of x / scale (one 32-bit division, one rounding to e4m3) and max|x| / 448, for rows with every
+    largest mantissa of bf16 (128 of them) next to every bf16 value of the ten octaves below, in which values
+    half-way between two e4m3 numbers occur; at the smallest and largest magnitudes of the type, too."""
+    torch.manual_seed(1)
+    mantissas = 1 + torch.arange(128) / 128
+    values = torch.cat([mantissas * 2.0 ** -e for e in range(10)])            # 1280
+    rows = torch.zeros(128, 6, 256)
+    for i in range(6):
+        some = values[214 * i:214 * (i + 1)]
+        rows[:, i, 1:1 + len(some)] = torch.minimum(some, mantissas[:, None])
+        rows[:, i, 0] = mantissas
+    rows = (rows * torch.where(torch.rand(rows.shape) < 0.5, -1.0, 1.0)).flatten(0, 1)
+    ups = [1.0, 2.0 ** -10, 2.0 ** 14] if dtype == torch.float16 else [1.0, 2.0 ** -125, 2.0 ** -117, 2.0 ** -60,
+                                                                       2.0 ** 100, 2.0 ** 126]
+    x = torch.cat([rows * up for up in ups]).to(dtype)
+    tokens = x.shape[0]
+    for dim in (256, 255):                                                     # rows in wide accesses, and not
+        part = x[:, :dim].reshape(1, tokens, 1, dim)
+        cache = nb.KVCache.allocate(-(-tokens // 64), 64, 1, dim, E4M3)
+        table = torch.arange(cache.key.shape[0], dtype=torch.int32, device="cuda").view(1, -1)
+        nb.kv_cache_write(cache, part.cuda(), -part.cuda(), table)
+        full = part[0, :, 0].float()
+        scale = torch.clamp_min(full.abs().amax(-1) / 448.0, 2.0 ** -126)
+        for pool, scales, sign in ((cache.key, cache.key_scale, 1.0), (cache.value, cache.value_scale, -1.0)):
+            assert torch.equal(scales.flatten()[:tokens].cpu(), scale)
+            want = (sign * full / scale[:, None]).to(E4M3)
+            got = pool.view(-1, dim)[:tokens].cpu()
+            assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
