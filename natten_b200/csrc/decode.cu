@@ -827,7 +827,8 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         float factor = 1.f;
         if (e > kUp - 126) {
           factor = __int_as_float((127 + kUp - e) << 23);
-          row_scale[x] *= __int_as_float((127 - kUp + e) << 23);
+          // (never 0, which the -inf of a token that is not attended must not meet: logits of that size are 0)
+          row_scale[x] = fmaxf(row_scale[x] * __int_as_float((127 - kUp + e) << 23), __int_as_float(1));
         }
         if constexpr (kSplit) {
           // e4m3 has no infinity: NaNs in its place, which only the tokens that the row attends bring to it

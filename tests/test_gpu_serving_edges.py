@@ -6,7 +6,6 @@ import pytest
 import torch
 
 import natten_b200 as nb
-import serving_reference as ref
 from test_gpu_decode import E4M3, TYPES, _check, _state
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +62,14 @@ def test_eight_bit_rows_are_divided_by_their_scale(dtype):
             want = (sign * full / scale[:, None]).to(E4M3)
             got = pool.view(-1, dim)[:tokens].cpu()
             assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [t for t in TYPES if t[0] != torch.float16])
+@pytest.mark.parametrize("heads", [4, 24])
+def test_logits_smaller_than_32_bits_hold(dtype, cache_dtype, heads):
+    """Queries of 2**-100 with a scale of 2**-60: every logit is nothing, every token that is there weighs
+    the same, and holes weigh nothing."""
+    q, cache, table, n = _state(dtype, cache_dtype, [90, 33], 2, heads, 2, 64, 16, spread=2.0 ** -100)
+    table[0, 1] = -1
+    _check(q, cache, table, n, scale=2.0 ** -60)
+    _check(q, cache, table, n, 20, scale=2.0 ** -60)
