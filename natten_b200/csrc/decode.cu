@@ -823,7 +823,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
         // The row times the power of two that brings its largest magnitude to [1, 2) (kSplit: [128, 256)), where
         // that power and its inverse are normal numbers.
         constexpr int kUp = kSplit ? 7 : 0;
-        const int e = min((__float_as_int(most) >> 23) - 127, 126);
+        const int e = min((__float_as_int(most) >> 23) - 127, kUp ? 127 : 126);
         float factor = 1.f;
         if (e > kUp - 126) {
           factor = __int_as_float((127 + kUp - e) << 23);

@@ -73,3 +73,15 @@ def test_logits_smaller_than_32_bits_hold(dtype, cache_dtype, heads):
     table[0, 1] = -1
     _check(q, cache, table, n, scale=2.0 ** -60)
     _check(q, cache, table, n, 20, scale=2.0 ** -60)
+
+
+@pytest.mark.parametrize("heads", [4, 24])
+def test_queries_near_the_largest_number(heads):
+    """bf16 queries of 2**127 and more on keys of about 2**-125."""
+    q, cache, table, n = _state(torch.bfloat16, E4M3, [90, 33], 2, heads, 2, 64, 16)
+    big = torch.finfo(torch.bfloat16).max
+    q = ((torch.rand(q.shape, device="cuda") * 0.5 + 0.5) * torch.sign(q.float()) * big).bfloat16()
+    key = (torch.randn(2, 90, 2, 64, device="cuda") * 2.0 ** -125).bfloat16()
+    value = torch.randn(2, 90, 2, 64, device="cuda").bfloat16()
+    nb.kv_cache_write(cache, key, value, table, counts=n)
+    _check(q, cache, table, n)
