@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ 
   const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
   const int group = threadIdx.x >> lanes_log2, groups = kThreads >> lanes_log2;
   const int b = blockIdx.x / a.tiles, t0 = (blockIdx.x - b * a.tiles) * a.tokens;
-  const int count = a.counts ? min(a.counts[b], a.T) : a.T;          // tokens that are moved
+  const int count = a.counts ? max(min(a.counts[b], a.T), 0) : a.T;  // tokens that are moved
   const int here = min(a.tokens, (kWrite ? count : a.T) - t0);       // rows of tokens t0 + [0, here)
   if (here <= 0) return;
   const int64_t start = a.start ? a.start[b] : 0;

@@ -85,3 +85,20 @@ def test_queries_near_the_largest_number(heads):
     value = torch.randn(2, 90, 2, 64, device="cuda").bfloat16()
     nb.kv_cache_write(cache, key, value, table, counts=n)
     _check(q, cache, table, n)
+
+
+@pytest.mark.parametrize("eight_bits", [False, True])
+def test_counts_far_below_zero(eight_bits):
+    """Nothing is written, and nothing read of the keys behind the call's tokens (whose number is no multiple of
+    a block's)."""
+    cache = nb.KVCache.allocate(40, 64, 2, 16, E4M3 if eight_bits else torch.bfloat16)
+    for t in cache:
+        if t is not None:
+            t.copy_(torch.ones(t.shape, device="cuda").to(t.dtype))
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40)
+    x = torch.randn(1, 2501, 2, 16, device="cuda").bfloat16()
+    for count in (-2 ** 31, -2 ** 31 + 1, -1):
+        n = torch.tensor([count], dtype=torch.int32, device="cuda")
+        nb.kv_cache_write(cache, x, x, table, counts=n)
+        assert all((t.float() == 1).all() for t in cache if t is not None)
+        assert not any(t.any() for t in nb.kv_cache_read(cache, table, 2501, counts=n))
