@@ -262,7 +262,7 @@ int launch(MoveArgs a, cudaStream_t stream) {
   const int64_t round = kThreads >> lanes_log2, all = (int64_t)a.B * a.T * a.heads / round;
   const int64_t rows = round * std::max<int64_t>(1, std::min<int64_t>(8, all / (8 * sms)));
   a.tokens = rows > a.heads ? (int)rows / a.heads : 1;
-  a.tiles = (a.T + a.tokens - 1) / a.tokens;
+  a.tiles = (int)(((int64_t)a.T + a.tokens - 1) / a.tokens);
   a.narrow = true;
   for (int w = 0; w < 2; ++w)
     for (int64_t stride : {a.token[w], a.head[w]}) a.narrow = a.narrow && stride >= 0 && stride <= 0x7fffffff;

@@ -102,3 +102,17 @@ def test_counts_far_below_zero(eight_bits):
         nb.kv_cache_write(cache, x, x, table, counts=n)
         assert all((t.float() == 1).all() for t in cache if t is not None)
         assert not any(t.any() for t in nb.kv_cache_read(cache, table, 2501, counts=n))
+
+
+def test_the_longest_read():
+    """2**31 - 1 tokens, the last number that is accepted: what is cached, then zeros to the end."""
+    cache = nb.KVCache.allocate(2, 8, 1, 1, torch.float16)
+    for t in cache[:2]:
+        t.copy_(torch.arange(1, 17, device="cuda").view(2, 8, 1, 1))
+    table = torch.tensor([[1, 0, -1]], dtype=torch.int32, device="cuda")
+    start = torch.tensor([3], dtype=torch.int32, device="cuda")
+    key, value = nb.kv_cache_read(cache, table, 2 ** 31 - 1, start)
+    want = torch.cat((torch.arange(12, 17), torch.arange(1, 9))).half().cuda()
+    for t in (key, value):
+        assert t.shape == (1, 2 ** 31 - 1, 1, 1) and torch.equal(t[0, :13, 0, 0], want)
+        assert not t[0, 13:].any()
