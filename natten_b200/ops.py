@@ -407,6 +407,10 @@ def rotary(query: Tensor, key: Optional[Tensor], axis_dims: List[int], theta: Li
     if positions is not None:
         positions = positions.contiguous()
     if query.numel() == 0:
+        if key is not None and key.numel() > 0:                # queries without heads
+            turned, _ = getattr(rotary, "raw", rotary)(key, None, axis_dims, theta, position_scale, origin,
+                                                       positions, interleaved, inverse)
+            return out[0], turned
         return out
     na_dim = query.dim() - 3
     with torch.cuda.device(query.device):

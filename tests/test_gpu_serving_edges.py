@@ -87,6 +87,20 @@ def test_queries_near_the_largest_number(heads):
     _check(q, cache, table, n)
 
 
+def test_rotary_turns_keys_beside_queries_without_heads():
+    torch.manual_seed(2)
+    key = torch.randn(2, 5, 3, 16, device="cuda").bfloat16()
+    query = torch.zeros(2, 5, 0, 16, device="cuda").bfloat16()
+    q, k = nb.rotary(query, key)
+    assert q.shape == query.shape and torch.equal(k, nb.rotary(key))
+    leaf, none = key.clone().requires_grad_(), query.clone().requires_grad_()
+    d = torch.randn_like(key)
+    want, = torch.autograd.grad(nb.rotary(leaf), leaf, d)
+    a, b = nb.rotary(none, leaf)
+    got = torch.autograd.grad((a, b), (none, leaf), (torch.zeros_like(a), d))
+    assert got[0].shape == query.shape and torch.equal(got[1], want)
+
+
 @pytest.mark.parametrize("eight_bits", [False, True])
 def test_counts_far_below_zero(eight_bits):
     """Nothing is written, and nothing read of the keys behind the call's tokens (whose number is no multiple of
