@@ -1445,7 +1445,7 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   const int rows = p->item_tokens * p->item_heads;
   if (p->rows_max == 16 && rows <= 8) p->rows_max = 8;
   else if (p->in_chunks && dtype == B200NA_F32 && rows <= 4) p->rows_max = rows <= 2 ? 2 : 4;
-  p->token_blocks = (T + p->item_tokens - 1) / p->item_tokens;
+  p->token_blocks = (int)(((int64_t)T + p->item_tokens - 1) / p->item_tokens);
   // a tile for each of a block's warps
   const int elem = elem_bytes(cache->dtype);
   p->step = kWarps * (p->in_chunks ? tile_keys((D <= 64 ? 64 : D <= 128 ? 128 : 256) * elem, elem) : 32);
@@ -1456,7 +1456,7 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   if (most > 0x7fffffff - 4096) return B200NA_ERR_UNSUPPORTED;
   if (kernel > 0 && most > (int64_t)kernel + p->item_tokens) most = (int64_t)kernel + p->item_tokens;
   p->unit = p->step;
-  while (B * p->items * (most / p->unit + 1) > 0x7fffffff && p->unit <= most) p->unit *= 2;
+  while (B * p->items * (most / p->unit + 1) > 0x7fffffff && p->unit <= most && p->unit < 1 << 30) p->unit *= 2;
   const int64_t units = B * p->items * (most / p->unit + 1);
   if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   const int held = p->in_chunks && D > 128 && elem > 1 ? kMostParts / 2 : kMostParts;   // (Tile::kBlocks)

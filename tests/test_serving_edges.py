@@ -1,0 +1,31 @@
+"""The serving operators at the edges of what they accept, on the host: sizes and strides at the C boundary and in
+the Python checks, before any CUDA call."""
+import ctypes
+
+import natten_b200._lib as L
+
+
+def _cache(pages=4, page_size=8, heads=1, head_dim=1, dtype=L.BF16, **strides):
+    c = L.KvCacheStruct()
+    for n, v in dict(key=1024, value=1024, pages=pages, page_size=page_size, heads=heads, head_dim=head_dim,
+                     dtype=dtype).items():
+        setattr(c, n, v)
+    for n in ("key_stride", "value_stride", "key_scale_stride", "value_scale_stride"):
+        getattr(c, n)[:] = strides.get(n, (page_size * heads * head_dim, heads * head_dim, head_dim))
+    return c
+
+
+def _workspace(c, T=1, Hq=1, max_pages=3, kernel=0, dilation=1, dtype=L.BF16):
+    return L.lib.b200na_na1d_decode_workspace(1, T, Hq, ctypes.byref(c), max_pages, kernel, dilation, dtype)
+
+
+def test_decode_counts_the_rows_of_very_many_tokens_in_64_bits():
+    """2^31 - 1 tokens are rounded up to whole items without wrapping around: more rows than a launch has are
+    refused, for every kernel."""
+    for T in (2 ** 31 - 1, 2 ** 31 - 7):
+        for c, dtype in ((_cache(), L.BF16), (_cache(head_dim=64), L.BF16), (_cache(head_dim=64, dtype=L.F32), L.F32)):
+            assert _workspace(c, T=T, dtype=dtype) == L.ERR_INVALID_ARGUMENT
+            assert _workspace(c, T=T, Hq=5, dtype=dtype) == L.ERR_INVALID_ARGUMENT
+    # one row an item (dilated, a query head for each key head): as many as fit 31 bits, if their keys do too
+    assert _workspace(_cache(), T=2 ** 31 - 1, dilation=2) >= 0
+    assert _workspace(_cache(page_size=2 ** 29), T=2 ** 31 - 1, dilation=2) == L.ERR_INVALID_ARGUMENT
