@@ -453,7 +453,7 @@ B200NA_API int b200na_rotary(const void* query, const void* key, void* query_out
  * dtype B200NA_F32 / F16 / BF16, or B200NA_E4M3 with one fp32 scale for each token and head: a row is
  * value * scale, scale = max(max|x| / 448, 2^-126); a row that holds a NaN or an infinity has the scale
  * NaN. The channels of a head are contiguous (head_dim <= 256); strides of page, token and head are in
- * elements of the pool (of the scales: in floats).
+ * elements of the pool (of the scales: in floats), 0 or more.
  */
 typedef struct {
   void* key;

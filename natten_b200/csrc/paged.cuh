@@ -101,6 +101,12 @@ inline int check_cache(const b200na_kv_cache* c, const int* table, int64_t table
     return B200NA_ERR_INVALID_ARGUMENT;
   }
   if (c->pages > 0 && (!c->key || !c->value)) return B200NA_ERR_INVALID_ARGUMENT;
+  // a place before the pool's first one would be taken for one that is not there
+  for (bool value : {false, true}) {
+    const PagedPool p = paged_pool(*c, value);
+    for (int64_t stride : {p.page, p.token, p.head, p.s_page, p.s_token, p.s_head})
+      if (stride < 0) return B200NA_ERR_INVALID_ARGUMENT;
+  }
   if (B > 0 && max_pages > 0 && !table) return B200NA_ERR_INVALID_ARGUMENT;
   return B200NA_OK;
 }

@@ -29,3 +29,24 @@ def test_decode_counts_the_rows_of_very_many_tokens_in_64_bits():
     # one row an item (dilated, a query head for each key head): as many as fit 31 bits, if their keys do too
     assert _workspace(_cache(), T=2 ** 31 - 1, dilation=2) >= 0
     assert _workspace(_cache(page_size=2 ** 29), T=2 ** 31 - 1, dilation=2) == L.ERR_INVALID_ARGUMENT
+
+
+def test_caches_whose_places_run_backwards_are_refused():
+    """Strides count from the first place of the pool upwards; the stride of an axis with one entry is not
+    looked at."""
+    ptr, rows = ctypes.c_void_p(1024), L.longs((1, 1, 1))
+    for name in ("key_stride", "value_stride", "key_scale_stride", "value_scale_stride"):
+        for axis in range(3):
+            strides = [64, 8, 4]
+            strides[axis] *= -1
+            c = _cache(heads=2, dtype=L.E4M3, **{name: strides})
+            c.key_scale = c.value_scale = 1024
+            calls = (
+                lambda: _workspace(c, Hq=2),
+                lambda: L.lib.b200na_kv_cache_write(ctypes.byref(c), ptr, ptr, 1, 0, L.BF16, rows, rows, ptr, 3, 3,
+                                                    None, None, None),
+                lambda: L.lib.b200na_kv_cache_read(ctypes.byref(c), ptr, ptr, 1, 0, L.BF16, ptr, 3, 3, None, None,
+                                                   None))
+            assert [f() for f in calls] == [L.ERR_INVALID_ARGUMENT] * 3
+            c.pages, c.page_size, c.heads = ((1, 8, 2), (4, 1, 2), (4, 8, 1))[axis]
+            assert [f() for f in calls] == [L.OK] * 3
