@@ -46,6 +46,12 @@ class KVCache(NamedTuple):
         return cls(*pools)
 
 
+def _check_sizes(name: str, t: Tensor) -> None:
+    if max(t.shape) >= 2 ** 31:
+        raise NotImplementedError(f"`{name}` must have less than 2**31 entries along every axis, got "
+                                  f"{tuple(t.shape)}.")
+
+
 def _expect_cache(cache: KVCache) -> None:
     if not isinstance(cache, KVCache):
         raise ValueError(f"Expected a KVCache, got {type(cache)}.")
@@ -63,6 +69,7 @@ def _check_cache(cache: KVCache) -> None:
         raise ValueError(f"A cache holds fp32, fp16, bf16 or e4m3, got {key.dtype}.")
     if min(key.shape[1:]) < 1:
         raise ValueError(f"A cache's pages, heads and channels cannot be empty, got {tuple(key.shape)}.")
+    _check_sizes("cache", key)
     if key.shape[-1] > MAX_HEAD_DIM:
         raise NotImplementedError(f"The cache takes head dims up to {MAX_HEAD_DIM}, got {key.shape[-1]}.")
     if key.shape[-1] > 1 and (key.stride(-1) != 1 or value.stride(-1) != 1):
@@ -82,6 +89,7 @@ def _check_rows(cache: KVCache, **tensors: Tensor) -> None:
         if t.dim() != 4 or t.shape[-1] != cache.key.shape[-1]:
             raise ValueError(f"`{name}` must be [batch, tokens, heads, {cache.key.shape[-1]}], got "
                              f"{tuple(t.shape)}.")
+        _check_sizes(name, t)
         if t.device != cache.key.device:
             raise ValueError(f"`{name}` must be on the cache's device, got {t.device}.")
         _check_dtype(cache, t.dtype, name)
@@ -100,6 +108,7 @@ def _table(cache: KVCache, page_table: Tensor, batch: Optional[int]) -> Tensor:
         raise ValueError("`page_table` must be an int32 tensor [batch, pages of a sequence] on the cache's "
                          f"device, got {page_table.dtype} {tuple(page_table.shape)} on "
                          f"{page_table.device}.")
+    _check_sizes("page_table", page_table)
     return page_table if page_table.stride(1) == 1 or page_table.shape[1] <= 1 else page_table.contiguous()
 
 

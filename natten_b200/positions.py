@@ -91,8 +91,9 @@ def rotary(query: Tensor, key: Optional[Tensor] = None, axis_dims: Optional[Sequ
         raise NotImplementedError(f"rotary() takes head dims up to {MAX_HEAD_DIM}, got {head_dim}.")
     if not isinstance(interleaved, bool):
         raise ValueError(f"`interleaved` must be a boolean, got {interleaved!r}.")
-    if max(query.shape) >= 2 ** 31:
-        raise NotImplementedError(f"rotary() takes axes of less than 2**31 tokens, got {tuple(query.shape)}.")
+    for t in (query, key):
+        if t is not None and max(t.shape) >= 2 ** 31:
+            raise NotImplementedError(f"rotary() takes axes of less than 2**31 entries, got {tuple(t.shape)}.")
     axes = query.dim() - 3
     if positions is not None:
         if positions.dtype not in ops.POSITION_CODE:

@@ -2,6 +2,10 @@
 the Python checks, before any CUDA call."""
 import ctypes
 
+import pytest
+import torch
+
+import natten_b200 as nb
 import natten_b200._lib as L
 
 
@@ -50,3 +54,25 @@ def test_caches_whose_places_run_backwards_are_refused():
             assert [f() for f in calls] == [L.ERR_INVALID_ARGUMENT] * 3
             c.pages, c.page_size, c.heads = ((1, 8, 2), (4, 1, 2), (4, 8, 1))[axis]
             assert [f() for f in calls] == [L.OK] * 3
+
+
+def test_sizes_beyond_31_bits_are_refused():
+    """Expanded tensors reach them without memory. (The C boundary takes 32-bit sizes: 2^32 + 3 is 3 there.)"""
+    far = 2 ** 32 + 3
+    x = torch.zeros(1, 1, 1, 2, dtype=torch.bfloat16)
+    cache = nb.KVCache.allocate(4, 8, 1, 2, device="cpu")
+    table, n = torch.zeros(1, 3, dtype=torch.int32), torch.tensor([3], dtype=torch.int32)
+    tokens, heads, batch = x.expand(1, far, 1, 2), x.expand(1, 1, far, 2), x.expand(far, 1, 1, 2)
+    wide = nb.KVCache(*(torch.zeros(1, 1, 1, 2, dtype=torch.bfloat16).expand(1, far, 1, 2) for _ in range(2)))
+    for call in (
+            lambda: nb.kv_cache_write(cache, tokens, tokens, table),
+            lambda: nb.kv_cache_write(cache, batch, batch, table.expand(far, 3)),
+            lambda: nb.kv_cache_read(cache, table.expand(far, 3), 1),
+            lambda: nb.kv_cache_read(cache, table[:, :1].expand(1, far), 1),
+            lambda: nb.kv_cache_read(wide, table, 1),
+            lambda: nb.na1d_decode(tokens, cache, table, n),
+            lambda: nb.na1d_decode(heads, cache, table, n),
+            lambda: nb.na1d_decode(batch, cache, table.expand(far, 3), n.expand(far)),
+            lambda: nb.rotary(x, heads), lambda: nb.rotary(heads), lambda: nb.rotary(tokens, tokens)):
+        with pytest.raises(NotImplementedError):
+            call()
