@@ -8,7 +8,7 @@ import torch
 from torch import Tensor
 
 from . import _native, ops
-from .functional import _native_eligible, _require_cuda
+from .functional import _native_eligible, _require_cuda, _wants_grad
 
 ROTARY_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_HEAD_DIM = 256
@@ -63,7 +63,8 @@ def rotary(query: Tensor, key: Optional[Tensor] = None, axis_dims: Optional[Sequ
     of axes from 1 to 3 (a flat sequence of text and image tokens can carry time, height and width).
 
     Returns new contiguous tensors: the query alone when there is no key, else (query, key). fp32, fp16
-    and bf16, head dims up to 256; differentiable in query and key, also twice."""
+    and bf16, head dims up to 256; differentiable in query and key, also twice (refused where
+    ``NATTEN_B200_DISABLE_TORCH_OPS=1`` leaves no registered operator to hold the formula)."""
     if _native_eligible():
         result = _native.rotary(query, key, axis_dims, theta, positions, origin, position_scale, interleaved)
         if result is not None:
@@ -110,6 +111,9 @@ def rotary(query: Tensor, key: Optional[Tensor] = None, axis_dims: Optional[Sequ
     how = check_rotary_args(axes, head_dim, axis_dims, theta, origin, position_scale)
     if positions is not None and any(how[3]):
         raise ValueError("`origin` belongs to positions that come from the layout; add it to `positions`.")
+    if not ops.USE_TORCH_OPS and _wants_grad(query, key):
+        raise NotImplementedError("rotary() has no gradient without registered operators "
+                                  "(NATTEN_B200_DISABLE_TORCH_OPS=1).")
     _require_cuda(query, key, positions)
     out = ops.rotary(query, key, *how, positions, interleaved, False)
     return out[0] if key is None else out

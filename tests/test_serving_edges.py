@@ -1,6 +1,9 @@
 """The serving operators at the edges of what they accept, on the host: sizes and strides at the C boundary and in
 the Python checks, before any CUDA call."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -76,3 +79,24 @@ def test_sizes_beyond_31_bits_are_refused():
             lambda: nb.rotary(x, heads), lambda: nb.rotary(heads), lambda: nb.rotary(tokens, tokens)):
         with pytest.raises(NotImplementedError):
             call()
+
+
+def test_rotary_does_not_detach_without_registered_operators():
+    """NATTEN_B200_DISABLE_TORCH_OPS=1 leaves no place for a gradient formula: the call says so."""
+    code = ("import torch, natten_b200 as nb\n"
+            "x = torch.zeros(1, 4, 2, 16)\n"
+            "for args in ((x.clone().requires_grad_(),), (x, x.clone().requires_grad_())):\n"
+            "    try:\n"
+            "        nb.rotary(*args)\n"
+            "    except NotImplementedError as e:\n"
+            "        print('refused', 'NATTEN_B200_DISABLE_TORCH_OPS' in str(e))\n"
+            "    with torch.no_grad():\n"
+            "        try:\n"
+            "            nb.rotary(*args)\n"
+            "        except RuntimeError as e:\n"
+            "            print(type(e).__name__)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "NATTEN_B200_DISABLE_TORCH_OPS": "1"})
+    assert done.returncode == 0, done.stderr
+    assert done.stdout.split("\n")[:-1] == ["refused True", "RuntimeError"] * 2      # (CPU tensors without gradients)
