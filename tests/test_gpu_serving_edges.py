@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import natten_b200 as nb
+import serving_reference as ref
 from test_gpu_decode import E4M3, TYPES, _check, _state
 
 pytestmark = pytest.mark.gpu
@@ -99,6 +100,83 @@ def test_rotary_turns_keys_beside_queries_without_heads():
     a, b = nb.rotary(none, leaf)
     got = torch.autograd.grad((a, b), (none, leaf), (torch.zeros_like(a), d))
     assert got[0].shape == query.shape and torch.equal(got[1], want)
+
+
+def _assert_holds(got, x):
+    """8-bit rows read back against what was written: half an e4m3 step of each value (at the row's scale the
+    smallest step is 2**-9), and two half steps of bf16 for products that torch splits differently."""
+    x = x.float()
+    scale = x.abs().amax(-1, keepdim=True) / 448
+    tol = torch.maximum(x.abs() * 2.0 ** -4, 2.0 ** -10 * scale) * 1.01 + 2 * 2.0 ** -8 * x.abs().amax(-1, keepdim=True)
+    assert ((got - x).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rotary_theta", [None, 1e4])
+@pytest.mark.parametrize("kernel_size,dilation", [(24, 1), (7, 4), (100, 1)])
+def test_steps_of_a_layer_over_an_eight_bit_cache(kernel_size, dilation, rotary_theta):
+    """The layer's steps against 64 bits on the cache as it was quantised: no tolerance for the 8 bits."""
+    torch.manual_seed(3)
+    B, N, heads, dim = 3, 120, 4, 32
+    layer = nb.NeighborhoodAttention1D(heads * dim, heads, kernel_size, 1, dilation, True,
+                                       rotary_theta=rotary_theta).cuda().bfloat16().eval()
+    x = torch.randn(B, N, heads * dim, device="cuda").bfloat16()
+    cache = nb.KVCache.allocate(60, 8, heads, dim, E4M3)
+    table = torch.randperm(60, device="cuda")[:B * 15].view(B, 15).int()
+    at = [60, 31, 45]
+    weight, bias = layer.proj.weight.detach().double().cpu(), layer.proj.bias.detach().double().cpu()
+    half = ref.HALF_STEP[torch.bfloat16]
+    with torch.no_grad():
+        q_all, k_all, v_all = layer._project(x)              # at the positions of the layout
+        layer.prefill(x[:, :60].contiguous(), cache, table, torch.tensor(at, dtype=torch.int32, device="cuda"))
+        for tokens in (1, 3, 1, 2):
+            rows = torch.stack([x[b, at[b]:at[b] + tokens] for b in range(B)])
+            q = torch.stack([q_all[b, at[b]:at[b] + tokens] for b in range(B)])
+            at = [n + tokens for n in at]
+            lengths = torch.tensor(at, dtype=torch.int32, device="cuda")
+            y = layer.decode(rows, cache, table, lengths).double().cpu()
+            key, value = nb.kv_cache_read(cache, table, max(at), dtype=torch.float32)
+            for b in range(B):
+                _assert_holds(key[b, :at[b]], k_all[b, :at[b]])
+                _assert_holds(value[b, :at[b]], v_all[b, :at[b]])
+            # the projection of a few rows may be summed in another order than that of all: its own queries
+            positions = (lengths[:, None] - tokens + torch.arange(tokens, device="cuda", dtype=torch.int32))[..., None]
+            own = layer._project(rows, positions if rotary_theta else None)[0]
+            assert (own.float() - q.float()).abs().max() <= 4 * half * q.float().abs().max()
+            cpu = nb.KVCache(*(t.cpu() for t in cache))
+            out, _, tol, _ = ref.decode(own.cpu(), cpu, table.cpu(), at, kernel_size, dilation, layer.scale, 2.0 ** -11)
+            out, tol = out.flatten(2), tol.flatten(2)
+            want = out @ weight.T + bias
+            # the attention's own error through the weights, the result's half step, and two more of the sum
+            # of magnitudes where torch adds partial sums in the type
+            over = tol @ weight.abs().T + half * want.abs() + 2 * half * (out.abs() @ weight.abs().T)
+            assert ((y - want).abs() <= over).all()
+            # (an attention of zeros would be told apart, for every token)
+            assert ((want - bias).abs() > 2 * over).any(-1).all()
+
+
+def test_a_run_over_an_eight_bit_cache():
+    """Rotary positions, writes and attention of one model step after the other, against 64 bits on the cache
+    as it was quantised."""
+    torch.manual_seed(9)
+    B, N, heads, heads_kv, dim, at = 2, 90, 4, 2, 64, 70
+    q, k, v = (torch.randn(B, N, h, dim, device="cuda").bfloat16() for h in (heads, heads_kv, heads_kv))
+    qr, kr = nb.rotary(q, k)
+    cache = nb.KVCache.allocate(30, 8, heads_kv, dim, E4M3)
+    table = torch.randperm(30, device="cuda")[:24].view(B, 12).int()
+    nb.kv_cache_write(cache, kr[:, :at], v[:, :at], table)
+    for tokens in (1, 1, 4, 1, 8, 1, 4):
+        start = torch.full((B,), at, dtype=torch.int32, device="cuda")
+        positions = (start[:, None] + torch.arange(tokens, device="cuda", dtype=torch.int32))[..., None]
+        qs, ks = nb.rotary(q[:, at:at + tokens], k[:, at:at + tokens], positions=positions)
+        nb.kv_cache_write(cache, ks, v[:, at:at + tokens], table, start)
+        at += tokens
+        assert torch.equal(qs, qr[:, at - tokens:at])
+        out, _ = _check(qs, cache, table, start + tokens, 32)
+        key, value = nb.kv_cache_read(cache, table, at, dtype=torch.float32)
+        _assert_holds(key, kr[:, :at])
+        _assert_holds(value, v[:, :at])
+        assert (out.float().abs() > 0.1).any(-1).all()
+    assert at == N
 
 
 @pytest.mark.parametrize("eight_bits", [False, True])
