@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 // sums and outputs are fp32. 8-bit rows are converted to fp16, which holds every e4m3 value, in registers. A key's scale multiplies its
 // logits; a value's scale goes into its weight as 2^(s_j + log2 scale_j - m'), with a running maximum m' of
 // its own, so that the largest of these weights is 1 whatever the scales are and fp16 loses only what is
-// 2^-24 of it. Queries are multiplied by a power of two that brings the row's largest to [1, 2), exactly.
+// 2^-24 of it. Queries on 8-bit keys are multiplied by a power of two that brings the row's largest to [1, 2); channels
+// below 2^-14 of it (bf16: 2^-17) are off by up to 2^-25 of it in fp16.
 template <class T> struct Half2Of;
 template <> struct Half2Of<__half> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -834,7 +835,9 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
           // e4m3 has no infinity: NaNs in its place, which only the tokens that the row attends bring to it
           if (!(most < INFINITY)) factor = __int_as_float(0x7fc00000);
           // A bf16 number is the sum of two e4m3 ones: the nearest one and what is left (four bits and sign,
-          // times 16). Row r0 of the instruction is the first, row r0 + 8 the second.
+          // times 16). Row r0 of the instruction is the first, row r0 + 8 the second. Nothing is lost of channels
+          // within 2^13 of the row's largest; what is left of smaller ones ends at e4m3's smallest step, which is
+          // 2^-21 of the largest channel at most (an 8-bit key is off by 2^-4 of itself).
 #pragma unroll
           for (int k = 0; k < kSteps; ++k) {
             float left[4];
@@ -901,7 +904,7 @@ decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
       const uint32_t keys = base + key_off;
       if constexpr (kSplit) {
         // 8-bit operands: the keys as they are, four times the rate of 16-bit ones (m16n8k32 4.5 cycles, the
-        // 16-bit m16n8k16 8 cycles) and no conversions. Both parts of the queries are exact, so are the products.
+        // 16-bit m16n8k16 8 cycles) and no conversions. The products of e4m3 numbers are exact.
 #pragma unroll
         for (int k = 0; k < kSteps / 2; ++k)
 #pragma unroll

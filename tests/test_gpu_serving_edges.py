@@ -179,6 +179,30 @@ def test_a_run_over_an_eight_bit_cache():
     assert at == N
 
 
+@pytest.mark.parametrize("heads", [4, 24])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("octaves", [12, 18])
+def test_query_channels_of_very_different_size(dtype, heads, octaves):
+    """8-bit keys that are zero in the query's largest channels, so that the small ones decide. Within 2**13 of
+    a row's largest channel nothing is lost of a bf16 query; below, and of fp16 queries, 2**-21 of the largest."""
+    q, cache, table, n = _state(dtype, E4M3, [90, 33], 2, heads, 2, 64, 16)
+    size = 2.0 ** (2 - octaves * torch.arange(64, device="cuda") / 63)
+    q = ((1 + torch.rand(q.shape, device="cuda")) * torch.sign(q.float()) * size).to(dtype)
+    key = torch.randn(2, 90, 2, 64, device="cuda").to(dtype)
+    key[..., :20] = 0
+    value = torch.randn(2, 90, 2, 64, device="cuda").to(dtype)
+    nb.kv_cache_write(cache, key, value, table, counts=n)
+    scale = 2.0 ** 4
+    out, lse = nb.na1d_decode(q, cache, table, n, scale=scale, return_lse=True)
+    cpu = nb.KVCache(*(t.cpu() for t in cache))
+    want, want_lse, tol, tol_lse = ref.decode(q.cpu(), cpu, table.cpu(), n.tolist(), 0, 1, scale, 2.0 ** -11)
+    lost = 0.0 if octaves <= 12 and dtype == torch.bfloat16 else 2.0 ** -21
+    key = nb.kv_cache_read(cache, table, 90, counts=n, dtype=torch.float32)[0]
+    logit = (lost * scale * q.float().abs().amax() * key.abs().sum(-1).max()).item()
+    ref.assert_close(out, want, tol + 4 * logit * 8.0)      # (values below 8)
+    ref.assert_close(lse, want_lse, tol_lse + logit)
+
+
 @pytest.mark.parametrize("eight_bits", [False, True])
 def test_counts_far_below_zero(eight_bits):
     """Nothing is written, and nothing read of the keys behind the call's tokens (whose number is no multiple of
