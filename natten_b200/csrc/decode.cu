@@ -3,11 +3,12 @@
 //
 //   s_j = scale * q . k_j,   out = sum_j exp(s_j - m) v_j / l,   m = max_j s_j,   l = sum_j exp(s_j - m)
 //
-// over the attended tokens j of one query row. Every attended key and value row is read once for all query
-// heads that share it and does about two products a byte and row: the memory's rate bounds it, so what
-// counts is that all SMs read all the time, whatever the sequences' lengths are.
+// over the attended tokens j of one query row. An attended key or value row is read once for the rows of an item
+// (below: up to 16), and again, mostly out of L2, where the query heads that share it times the new tokens are more.
+// It does about two products a byte and row: the memory's rate bounds it, so what counts is that all SMs read
+// all the time, whatever the sequences' lengths are.
 //
-// Work: an item is one sequence, one key/value head and up to 16 (CUDA cores: 8) rows, which are the heads
+// Work: an item is one sequence, one key/value head and up to 16 (fp32 and CUDA cores: 8) rows, which are the heads
 // of the group times neighbouring query tokens. Its keys are cut into units, a tile for each warp of a block.
 // Lengths are read on the device, so the host waits for nothing and a captured launch follows them.
 //  - Few units at most (a window, a short table): a cluster of 1, 2, 4 or 8 blocks has an item, and joins its
@@ -508,8 +509,9 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(const __grid_cons
 // fragments that ldmatrix takes out of the copied rows is enough (a 16-key bf16 tile: 32 of them, 256 of the
 // 1365 cycles that its 8 KB take at the copy rate); tcgen05 would want 128-row tiles and the probabilities in
 // shared memory or TMEM for the same bytes. Measured: 64 sequences of 4 x 128 channels behind 2048 tokens, 259 MB
-// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 70 us (68 %: the conversions
-// and exponentials of a 32-key tile take about as many issue slots as its bytes take cycles).
+// in 49 us (5.3 TB/s, 80 % of the copy rate); 16 whole 8-bit contexts, 312 MB in 71 us (67 %; 46 % of issue slots and
+// 29 % of the tensor pipe in use: the two warps of a scheduler wait for their own chains of products, conversions,
+// maxima and exponentials).
 //
 // Weights are rounded to the values' 16-bit type for the second product, like in the prefill kernels; maxima,
 // sums and outputs are fp32. 8-bit rows are converted to fp16, which holds every e4m3 value, in registers. A key's scale multiplies its
@@ -1464,10 +1466,19 @@ int make_plan(Plan* p, int B, int T, int Hq, const b200na_kv_cache* cache, int m
   if (units > 0x7fffffff) return B200NA_ERR_INVALID_ARGUMENT;
   const int held = p->in_chunks && D > 128 && elem > 1 ? kMostParts / 2 : kMostParts;   // (Tile::kBlocks)
   p->parts = (int)(units < held ? (units < 1 ? 1 : units) : held);
-  // Clusters of the largest size that leaves every block a place of its own, where a block's share is bounded.
-  // Against ranges and their join (us): 64 sequences, 4 heads, window 2048 (33 units) 49.5 / 57.6, window 512
-  // (9) 18.9 / 29.0; 1 sequence, window 2048 (33 over 8 blocks) 12.5 / 26.8; 4 sequences of 1000 to 8190 tokens (128
-  // over 8) 23.0 / 33.3. Beyond, ranges are right: lengths may differ by more than what the join costs.
+  // Clusters of the largest size that leaves every block a place of its own (of one block where the items alone
+  // have none), where a block's share is bounded. Against ranges and their join (us; bf16, 4 heads of 128 channels, units
+  // of 64 keys):
+  //  - equal lengths, a place for each block: 256 items of 33 units (window 2048) 47 / 53; 16 sequences, 10, 20 and 40
+  //    units a block 23 / 27, 35 / 39, 60 / 64; 64 sequences, 20, 40 and 80 units 33 / 38, 58 / 63, 107 / 114
+  //  - lengths from almost nothing to the table's: 64 sequences, 10, 20, 40 and 80 units a block 17 / 23, 27 / 34,
+  //    46 / 46, 82 / 69; 16 sequences, 5, 10, 20 and 40 units 12.6 / 15.1, 19 / 19, 30 / 29, 50 / 42
+  //  - more items than places, 33 units each: 300 items 77 / 61, 360 84 / 71, 440 86 / 85, 512 90 / 96, 592 103 / 106,
+  //    680 129 / 124, 1024 176 / 178
+  //  - few items, so that eight blocks each leave places unused: 4 sequences, 4, 10, 20 and 40 units a block 12.5 / 12.9,
+  //    18.9 / 17.1, 29.5 / 27.2, 48 / 40, of lengths that differ 8 times 18 / 17 (10), 28 / 22 (20), 46 / 31 (40)
+  // So 40 is where uneven lengths take what the join costs, with items that fill the GPU. A little above 296 items, and
+  // with a few long sequences, ranges would take up to a third less.
   const int64_t item_units = most / p->unit + 1, item_count = B * p->items;
   p->cluster = 1;
   while (p->cluster < 8 && p->cluster < item_units && item_count * p->cluster * 2 <= held) p->cluster *= 2;

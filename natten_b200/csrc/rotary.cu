@@ -5,7 +5,8 @@
 //
 // Angles: a far position times a frequency needs more than 24 bits before it is reduced to one turn, so
 // position * (f / 2 pi) is formed and reduced in fp64 and only the fraction of a turn goes to the fp32
-// sincospi. A block works the angles of its tokens out once, into shared memory, and its threads keep their
+// sincospi. An angle is off by 2e-15 of itself at most (the frequency's rounding and the product's): nothing in fp32 up
+// to about 2^25, 1e-5 at 2^32. A block works the angles of its tokens out once, into shared memory, and its threads keep their
 // columns' cosines and sines while they go through the heads of queries and keys, of several batch entries where
 // these stand at the same places. The rest is a stream: every element is read once and written once.
 #include <algorithm>
@@ -40,9 +41,10 @@ struct RotaryArgs {
 // neighbours. A thread keeps its column of the rows, so that what depends on it is worked out once.
 template <class T, int kVec, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  // Rows that a thread has under way: about 96 bytes. A training step on 15 x 30 x 52 tokens of 12 + 12 heads
-  // with 1, 2, 3, 4, 6 rows of 16 bytes: 78, 64, 67, 68, 60 us (58 now; a video of 32 x 48 x 80 tokens, 24 + 24 heads
-  // of 128 channels, 3.0 GB: 461 us, the copy rate).
+  // Rows that a thread has under way: about 96 bytes. Both launches of a training step on 15 x 30 x 52 tokens of 12 + 12
+  // heads, as a replayed graph, with 1, 2, 3, 4, 6 rows of 16 bytes: 78, 64, 67, 68, 60 us (58 now; calls from the host
+  // take 73 to 77, autograd's pace). A video of 32 x 48 x 80 tokens, 24 + 24 heads of 128 channels, 3.0 GB: 462 us, the
+  // copy rate; 12 + 12 heads in fp32, the same bytes: 460 us.
   constexpr int kRowBytes = 2 * kVec * (int)sizeof(T), kUnroll = kRowBytes >= 32 ? 3 : 6;
   extern __shared__ __align__(16) float cs[];                 // [block_tokens][cosines, sines][stride]
   __shared__ int64_t in_at[2][kMostTokens], out_at[2][kMostTokens];   // offsets of the tokens' first head

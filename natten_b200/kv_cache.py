@@ -24,6 +24,8 @@ MAX_HEAD_DIM = 256
 class KVCache(NamedTuple):
     """Pools of pages. With ``torch.float8_e4m3fn`` pools, ``key_scale`` and ``value_scale`` (fp32,
     ``[pages, page_size, heads_kv]``) hold one scale for each token and head; otherwise they are None.
+    Scales are what `kv_cache_write` leaves there, 2**-126 or more, or NaN: attention works with a value
+    scale's logarithm.
 
     Any strides with contiguous channels will do (a ``[pages, heads, page_size, head_dim]`` pool is passed
     as its transpose). Slots that no token was written to are never read."""
@@ -134,7 +136,7 @@ def kv_cache_write(cache: KVCache, key: Tensor, value: Tensor, page_table: Tenso
     Token t of sequence b goes to position ``start[b] + t`` (``t`` without ``start``), if ``t <
     counts[b]`` (all without ``counts``): what lies behind a padded sequence's tokens stays as it was. An
     8-bit cache quantises as it is written: ``scale = max(max|x| / 448, 2**-126)`` for each token and head,
-    ``x / scale`` rounded to the nearest e4m3; a row that holds a NaN or an infinity reads back as NaN.
+    ``x / scale`` (both 32-bit divisions) rounded to the nearest e4m3; a row that holds a NaN or an infinity reads back as NaN.
 
     Positions that are negative, behind the table, or on a table entry outside ``[0, pages)`` are dropped.
     The slots of one call must be different ones: of two tokens on the same slot, which one (or a mixture)
@@ -163,7 +165,8 @@ def kv_cache_read(cache: KVCache, page_table: Tensor, length: int, start: Option
                   counts: Optional[Tensor] = None,
                   dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """Reads tokens back: contiguous ``[batch, length, heads_kv, head_dim]`` keys and values, e.g. a cached
-    prefix that a new chunk attends with `attention`.
+    prefix that a new chunk attends with `attention`. That takes no lengths, and a key of zeros has a weight
+    like any other: read prefixes of equal length together, others one by one.
 
     Row t of sequence b is the token at ``start[b] + t`` (``t`` without ``start``); rows ``t >= counts[b]``
     and tokens that are on no page are zeros. ``dtype`` is the cache's, or fp32, fp16 or bf16 for an 8-bit
