@@ -37,8 +37,9 @@ __global__ void __launch_bounds__(256) merge_kernel(const T* o0,   // o may alia
     const int64_t row = idx / chunks;
     const int chunk = (int)(idx - row * chunks);
     const float a = l0[row], b = l1[row];
-    // sigmoid(b - a), written so that neither branch overflows
-    const float dlt = b - a;
+    // sigmoid(b - a), written so that neither branch overflows; 0 where the second result is empty (the first may
+    // be empty, too: no difference of infinities)
+    const float dlt = b == -INFINITY ? -INFINITY : b - a;
     const float e = expf(-fabsf(dlt));
     const float sg = dlt >= 0.f ? 1.f / (1.f + e) : e / (1.f + e);
     const int64_t base = row * D + (int64_t)chunk * kElems;

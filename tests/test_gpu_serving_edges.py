@@ -232,3 +232,20 @@ def test_the_longest_read():
     for t in (key, value):
         assert t.shape == (1, 2 ** 31 - 1, 1, 1) and torch.equal(t[0, :13, 0, 0], want)
         assert not t[0, 13:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 33])
+def test_rows_that_attend_nothing_in_either_part_merge_to_zeros(dtype, dim):
+    """Attention over two caches joined: a place that a sequence does not have is empty in both."""
+    q, one, table, n = _state(dtype, dtype, [1, 40, 0], 3, 4, 2, dim, 16)
+    _, two, other, m = _state(dtype, dtype, [2, 0, 0], 3, 4, 2, dim, 16, seed=1)
+    a, la = nb.na1d_decode(q, one, table, n, return_lse=True)
+    b, lb = nb.na1d_decode(q, two, other, m, return_lse=True)
+    for x, y, lx, ly in ((a, b, la, lb), (b, a, lb, la)):
+        out, lse = nb.merge_attentions([x, y], [lx, ly])
+        empty = torch.isneginf(la) & torch.isneginf(lb)
+        assert empty[0, 0].all() and empty[2].all() and int(empty.sum()) == 4 * 4
+        assert not out[empty].any() and torch.isneginf(lse[empty]).all()
+        assert torch.isfinite(out).all() and torch.isfinite(lse[~empty]).all()
+        assert torch.equal(out[1], a[1]) and torch.equal(lse[1], la[1])        # (nothing in the other part)
