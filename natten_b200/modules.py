@@ -17,7 +17,7 @@ from torch.nn.modules.module import _has_any_global_hook
 from . import _native
 from .checks import check_all_args
 from .functional import _native_eligible, attention, neighborhood_attention_generic
-from .kv_cache import KVCache, _refuse_grad, kv_cache_write, na1d_decode
+from .kv_cache import KVCache, _expect_cache, _per_sequence, _refuse_grad, kv_cache_write, na1d_decode
 from .positions import check_rotary_args, rotary
 
 
@@ -130,9 +130,17 @@ class NeighborhoodAttention1D(NeighborhoodAttentionGeneric):
                 counts: Optional[Tensor] = None) -> Tensor:
         """The layer on whole prompts ``[batch, tokens, embed_dim]``, whose keys and values go into the
         cache: token t of sequence b at position t, if ``t < counts[b]`` (prompts padded at their end;
-        all without ``counts``). The rows of the output behind a prompt mean nothing. A dilated layer needs
+        all without ``counts``). What lies behind a prompt may be anything, and the rows of the output there
+        mean nothing. A dilated layer needs
         as many tokens as its window spans, like `forward`."""
         self._check_serving(x)
+        _expect_cache(cache)
+        counts = _per_sequence(cache, counts, x.shape[0], "counts")
+        if counts is not None:
+            # What lies behind a prompt may be anything: a NaN there has weight 0 for the prompt's rows, but the
+            # tensor cores' products with 0 would keep it.
+            behind = torch.arange(x.shape[1], device=x.device) >= counts[:, None]
+            x = x.masked_fill(behind[..., None], 0.0)
         q, k, v = self._project(x)
         _refuse_grad("prefill()", q, k, v)
         if x.shape[1] < self.kernel_size[0] and self.dilation[0] == 1:      # a window over all of it

@@ -249,3 +249,34 @@ def test_rows_that_attend_nothing_in_either_part_merge_to_zeros(dtype, dim):
         assert not out[empty].any() and torch.isneginf(lse[empty]).all()
         assert torch.isfinite(out).all() and torch.isfinite(lse[~empty]).all()
         assert torch.equal(out[1], a[1]) and torch.equal(lse[1], la[1])        # (nothing in the other part)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,kernel_size,dilation,tokens", [(64, 24, 1, 200), (64, 7, 4, 200), (128, 100, 1, 90),
+                                                             (33, 64, 1, 200)])
+def test_what_lies_behind_a_prompt_does_not_reach_it(dtype, dim, kernel_size, dilation, tokens):
+    """Padding that is not finite (memory that nothing was written to) changes no bit of the prompts' rows and of the
+    cache."""
+    torch.manual_seed(4)
+    layer = nb.NeighborhoodAttention1D(2 * dim, 2, kernel_size, 1, dilation, True,
+                                       rotary_theta=None if dim % 2 else 1e4).cuda().to(dtype).eval()
+    counts = [tokens // 2, 17, tokens, 0]
+    x = torch.randn(4, tokens, 2 * dim, device="cuda").to(dtype)
+    n = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    table = torch.arange(56, device="cuda").int().view(4, 14)
+    got = []
+    for pad in (None, math.nan, math.inf):
+        z = x.clone()
+        for b in range(4):
+            if pad is not None:
+                z[b, counts[b]:] = pad
+        given = z.clone()
+        cache = nb.KVCache.allocate(56, 16, 2, dim, dtype)
+        with torch.no_grad():
+            y = layer.prefill(z, cache, table, n)
+        assert torch.equal(z.nan_to_num(7.0), given.nan_to_num(7.0))
+        rows = torch.cat([y[b, :counts[b]] for b in range(4)])
+        got.append((rows, *nb.kv_cache_read(cache, table, tokens, counts=n)))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    assert torch.isfinite(got[0][0]).all()
