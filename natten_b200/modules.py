@@ -131,8 +131,7 @@ class NeighborhoodAttention1D(NeighborhoodAttentionGeneric):
         """The layer on whole prompts ``[batch, tokens, embed_dim]``, whose keys and values go into the
         cache: token t of sequence b at position t, if ``t < counts[b]`` (prompts padded at their end;
         all without ``counts``). What lies behind a prompt may be anything, and the rows of the output there
-        mean nothing. A dilated layer needs
-        as many tokens as its window spans, like `forward`."""
+        mean nothing. A dilated layer needs as many tokens as its window spans, like `forward`."""
         self._check_serving(x)
         _expect_cache(cache)
         counts = _per_sequence(cache, counts, x.shape[0], "counts")
